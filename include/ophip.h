@@ -495,6 +495,120 @@ OPHIP_API int ophip_attention_kv_cached_launch(const ophip_attention_kv_cached *
                                                const ophip_queue_alloc *queue_alloc);
 OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
 
+/* ---- a paged cache (no counterpart in the reference, whose cache is one buffer per sequence) ------------- */
+/* The three operators below make up a serving step over a cache that is cut into pages, for a packed batch of
+ * sequences of unlike lengths.
+ *   k_cache, v_cache [pages, nkvh, page, dh]: any strides, so either order of heads and tokens inside a page;
+ *                    `page` tokens (any number) to a page.
+ *   page_table [nseq, cols] u32 or i32: key j of sequence s is row j % page of page page_table[s, j / page].
+ *                    Entries behind a sequence's last page are not read.
+ *   q_start [nseq + 1], kv_len [nseq] u32 or i32: sequence s has the new tokens q_start[s] .. q_start[s + 1] - 1 of
+ *                    the batch's nt (none is fine) and kv_len[s] keys, the new ones included: new token i of n is key
+ *                    kv_len[s] - n + i.  Tokens in front of the first and behind the last sequence belong to none: their
+ *                    rows are neither read nor written.
+ * Table, starts and lengths are device data that may change between replays of a recorded launch.  The kernels bound
+ * what they take from them: token numbers by nt, lengths by cols * page; a page number that is none of the cache's
+ * gets nothing written to, and reads as some page of the cache.  Wrong data gives wrong rows, not stray accesses.
+ * Types: f16, bf16, f32, one for all tensors of a call.  dh up to 512. */
+
+/* attention of the new tokens over the cache: o = softmax(scale * q . k^T) . v, q and o [nh, nt, dh], nh a multiple of
+ * nkvh (query head h reads kv head h / (nh / nkvh)).  With OPHIP_MASK_CAUSAL new token i of n sees the keys up to its
+ * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero.  q is left alone; o may be q itself
+ * (the same view), otherwise it must not overlap q or the caches (ArgsNotSupport).
+ * Accumulation in f32, one rounding of the result. */
+typedef struct ophip_attention_paged_args {
+    ophip_tensor_layout q_layout;
+    const void *q_base;
+    ophip_tensor_layout k_cache_layout;
+    const void *k_cache_base;
+    ophip_tensor_layout v_cache_layout;
+    const void *v_cache_base;
+    ophip_tensor_layout o_layout;
+    void *o_base;
+    ophip_tensor_layout page_table_layout;
+    const void *page_table_base;
+    ophip_tensor_layout q_start_layout;
+    const void *q_start_base;
+    ophip_tensor_layout kv_len_layout;
+    const void *kv_len_base;
+    uint8_t mask; /* ophip_attn_mask */
+    float scale;  /* 1 / sqrt(dh), usually */
+} ophip_attention_paged_args;
+typedef struct ophip_attention_paged ophip_attention_paged;
+OPHIP_API int ophip_attention_paged_create(ophip_device *dev, ophip_attention_paged **out);
+OPHIP_API int ophip_attention_paged_scheme(ophip_attention_paged *op, const ophip_attention_paged_args *args,
+                                           size_t max_workspace_size, size_t *workspace_size);
+OPHIP_API int ophip_attention_paged_launch(const ophip_attention_paged *op, const ophip_attention_paged_args *args,
+                                           void *workspace, size_t workspace_len,
+                                           const ophip_queue_alloc *queue_alloc);
+OPHIP_API void ophip_attention_paged_destroy(ophip_attention_paged *op);
+
+/* The new tokens' k and v [nkvh, nt, dh] into the cache, k rotated by rope (adjacent pairs, angle
+ * p * theta^(-2 i / dh)) on the way; theta = 0: as they are, and p is not read.  p [nt] u32, u64, i32 or i64 holds the
+ * tokens' positions, none negative.  A token whose key number is negative (kv_len less than the number of new tokens)
+ * is not written.  k and v must not overlap the caches (ArgsNotSupport); two tokens with the same place in the cache
+ * leave either one's row.  The angles are taken in f64: rope's, to f32 accuracy at any position. */
+typedef struct ophip_kv_append_paged_args {
+    ophip_tensor_layout k_layout;
+    const void *k_base;
+    ophip_tensor_layout v_layout;
+    const void *v_base;
+    ophip_tensor_layout p_layout;
+    const void *p_base;
+    ophip_tensor_layout k_cache_layout;
+    void *k_cache_base;
+    ophip_tensor_layout v_cache_layout;
+    void *v_cache_base;
+    ophip_tensor_layout page_table_layout;
+    const void *page_table_base;
+    ophip_tensor_layout q_start_layout;
+    const void *q_start_base;
+    ophip_tensor_layout kv_len_layout;
+    const void *kv_len_base;
+    float theta;
+} ophip_kv_append_paged_args;
+typedef struct ophip_kv_append_paged ophip_kv_append_paged;
+OPHIP_API int ophip_kv_append_paged_create(ophip_device *dev, ophip_kv_append_paged **out);
+OPHIP_API int ophip_kv_append_paged_scheme(ophip_kv_append_paged *op, const ophip_kv_append_paged_args *args,
+                                           size_t max_workspace_size, size_t *workspace_size);
+OPHIP_API int ophip_kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_append_paged_args *args,
+                                           void *workspace, size_t workspace_len,
+                                           const ophip_queue_alloc *queue_alloc);
+OPHIP_API void ophip_kv_append_paged_destroy(ophip_kv_append_paged *op);
+
+/* rms_norm of each query and key head followed by rope, in one launch:
+ * y[t, h, :] = rope(x[t, h, :] / sqrt(mean(x[t, h, :]^2) + epsilon) * w, p[t]) with x = q, w = qw, y = qy and
+ * x = k, w = kw, y = ky.  q, qy [nt, nh, dh], k, ky [nt, nkh, dh] (either may have no heads), dh even and contiguous;
+ * qw, kw [dh] of the rows' type or f32; p and theta as in kv_append_paged (theta = 0: the norms alone).
+ * qy may be q and ky may be k (the same view); otherwise a y that overlaps its x is ArgsNotSupport, and qy must not
+ * share elements with k or ky. */
+typedef struct ophip_qk_norm_rope_args {
+    ophip_tensor_layout qy_layout;
+    void *qy_base;
+    ophip_tensor_layout q_layout;
+    const void *q_base;
+    ophip_tensor_layout qw_layout;
+    const void *qw_base;
+    ophip_tensor_layout ky_layout;
+    void *ky_base;
+    ophip_tensor_layout k_layout;
+    const void *k_base;
+    ophip_tensor_layout kw_layout;
+    const void *kw_base;
+    ophip_tensor_layout p_layout;
+    const void *p_base;
+    float epsilon;
+    float theta;
+} ophip_qk_norm_rope_args;
+typedef struct ophip_qk_norm_rope ophip_qk_norm_rope;
+OPHIP_API int ophip_qk_norm_rope_create(ophip_device *dev, ophip_qk_norm_rope **out);
+OPHIP_API int ophip_qk_norm_rope_scheme(ophip_qk_norm_rope *op, const ophip_qk_norm_rope_args *args,
+                                        size_t max_workspace_size, size_t *workspace_size);
+OPHIP_API int ophip_qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_args *args,
+                                        void *workspace, size_t workspace_len,
+                                        const ophip_queue_alloc *queue_alloc);
+OPHIP_API void ophip_qk_norm_rope_destroy(ophip_qk_norm_rope *op);
+
 /* ---- layer_norm: layer_norm/args.rs:7-55 ----------------------------------- */
 /* y[n,d] = (x - mean) * scale / (std + epsilon) + bias, std = sqrt(mean(x^2) - mean^2)
  * (layer_norm/common_cpu/mod.rs:127-147).  (scale/bias, x/y): any pairing of f16, bf16 and f32, and (f64, f64)

@@ -1,0 +1,448 @@
+// The operators of a serving step over a paged cache: attention_paged, kv_append_paged and qk_norm_rope.  They have no
+// counterpart in the reference crate, whose cache is one buffer per sequence (attention_kv_cached/args.rs:8-30) and whose
+// operators take one sequence at a time; names, layouts, verbs and errors follow the crate's operators.
+#include <algorithm>
+#include <cmath>
+
+#include "../kernels/params.h"
+#include "handle.hpp"
+
+using namespace ophip;
+
+namespace {
+
+void expect_index_type(uint64_t dt, const char *name) {
+    if (dt != OPHIP_DT_U32 && dt != OPHIP_DT_I32) throw type_not_support(std::string(name) + " must be 32-bit integers");
+}
+void expect_position_type(uint64_t dt) {
+    if (dt != OPHIP_DT_U32 && dt != OPHIP_DT_U64 && dt != OPHIP_DT_I32 && dt != OPHIP_DT_I64) throw type_not_support("p must be 32 or 64-bit integers");
+}
+void expect_element_type(uint64_t dt) {
+    if (dt != OPHIP_DT_F16 && dt != OPHIP_DT_BF16 && dt != OPHIP_DT_F32) throw type_not_support("f16, bf16 and f32 are supported");
+}
+int type_index(uint64_t dt) { return dt == OPHIP_DT_F16 ? 0 : dt == OPHIP_DT_BF16 ? 1 : 2; }
+
+// every stride known and a whole number of elements
+void expect_strides(const ophip_tensor_layout &l, const char *name) {
+    const ptrdiff_t unit = (ptrdiff_t)ophip_dtype_nbytes(l.dt);
+    for (uint64_t i = 0; i < l.ndim; ++i)
+        if (static_of(l.strides[i]) % unit != 0) throw strides_not_support(std::string("misaligned strides of ") + name);
+}
+// elements adjacent, everything else on 16-byte boundaries
+bool vector_rows(const ophip_tensor_layout &l, const void *base) {
+    if (!aligned16(base) || l.strides[l.ndim - 1] != (ptrdiff_t)ophip_dtype_nbytes(l.dt)) return false;
+    for (uint64_t i = 0; i + 1 < l.ndim; ++i)
+        if (!mult16(l.strides[i])) return false;
+    return true;
+}
+
+// Whether the address ranges two views reach do not meet (an empty view reaches nothing).
+bool apart(const ophip_tensor_layout &a, const void *a_base, const ophip_tensor_layout &b, const void *b_base) {
+    auto span = [](const ophip_tensor_layout &l, const void *base) {
+        const char *lo = static_cast<const char *>(base), *hi = lo + ophip_dtype_nbytes(l.dt);
+        for (uint64_t i = 0; i < l.ndim; ++i) {
+            if (l.shape[i] == 0) return std::pair<const char *, const char *>(nullptr, nullptr);
+            const ptrdiff_t reach = (ptrdiff_t)(l.shape[i] - 1) * l.strides[i];
+            (reach < 0 ? lo : hi) += reach;
+        }
+        return std::pair<const char *, const char *>(lo, hi);
+    };
+    const auto x = span(a, a_base), y = span(b, b_base);
+    return x.first == x.second || y.first == y.second || x.second <= y.first || y.second <= x.first;
+}
+bool same_view(const ophip_tensor_layout &a, const void *a_base, const ophip_tensor_layout &b, const void *b_base) {
+    if (a_base != b_base) return false;
+    for (uint64_t i = 0; i < a.ndim; ++i)
+        if (a.shape[i] > 1 && a.strides[i] != b.strides[i]) return false;
+    return true;
+}
+
+// theta as rope has it; 0: no rotation
+bool rotation(float theta, size_t dh, double *freq_step) {
+    const float t = static_of(theta);
+    if (!(t >= 0.f)) throw args_not_support("theta must not be negative");
+    if (t == 0.f) return false;
+    if (dh % 2) throw shape_not_support("rotation needs an even head dimension");
+    *freq_step = std::log2((double)t) / (double)(dh / 2);
+    return true;
+}
+
+constexpr size_t MAX_HEAD = 512;         // elements of a head
+constexpr size_t MAX_INDEX = 0x7fffffffu;
+
+// ---- the batch: page table [nseq, cols], first tokens [nseq + 1], lengths [nseq], cache [pages, nkvh, page, dh]
+struct BatchMeta {
+    size_t nseq, cols, npages, nkvh, page;
+};
+BatchMeta batch_meta(const ophip_tensor_layout &k_cache, const ophip_tensor_layout &v_cache, const ophip_tensor_layout &table,
+                     const ophip_tensor_layout &q_start, const ophip_tensor_layout &kv_len) {
+    expect_rank(k_cache, "k_cache", 4);
+    expect_rank(v_cache, "v_cache", 4);
+    expect_rank(table, "page_table", 2);
+    expect_rank(q_start, "q_start", 1);
+    expect_rank(kv_len, "kv_len", 1);
+    expect_index_type(table.dt, "page_table");
+    expect_index_type(q_start.dt, "q_start");
+    expect_index_type(kv_len.dt, "kv_len");
+    BatchMeta m;
+    const size_t starts = q_start.shape[0];
+    if (starts == 0) throw shape_mismatch("q_start has one value more than there are sequences");
+    m.nseq = dim_distinct({table.shape[0], kv_len.shape[0], is_dyn(starts) ? starts : starts - 1});
+    m.cols = table.shape[1];
+    m.npages = dim_distinct({k_cache.shape[0], v_cache.shape[0]});
+    m.nkvh = dim_distinct({k_cache.shape[1], v_cache.shape[1]});
+    m.page = dim_distinct({k_cache.shape[2], v_cache.shape[2]});
+    return m;
+}
+PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout &table, const void *table_base, const ophip_tensor_layout &q_start,
+                        const void *q_start_base, const ophip_tensor_layout &kv_len, const void *kv_len_base) {
+    const size_t page = static_of(m.page), npages = static_of(m.npages), nseq = static_of(m.nseq);
+    if (page == 0) throw shape_not_support("a page of no tokens");
+    const size_t cols = npages ? static_of(m.cols) : 0;  // (no pages: no keys)
+    if (nt > MAX_INDEX || nseq >= MAX_INDEX || npages > MAX_INDEX || page > MAX_INDEX || (cols && page > MAX_INDEX / cols))
+        throw shape_not_support("batch or cache too large");
+    expect_strides(table, "page_table");
+    expect_strides(q_start, "q_start");
+    expect_strides(kv_len, "kv_len");
+    if (!q_start_base || !kv_len_base || (cols && !table_base)) throw args_not_support("null base address");
+    PagedBatch b{};
+    b.table = table_base;
+    b.q_start = q_start_base;
+    b.kv_len = kv_len_base;
+    b.t_row = table.strides[0], b.t_col = table.strides[1], b.s_step = q_start.strides[0], b.l_step = kv_len.strides[0];
+    b.nseq = (uint32_t)nseq, b.nt = (uint32_t)nt, b.cols = (uint32_t)cols, b.npages = (uint32_t)npages;
+    b.page = make_fastdiv((uint32_t)page);
+    return b;
+}
+
+}  // namespace
+
+// ============================================================== attention_paged ===
+
+struct ophip_attention_paged : OpBase {
+    hipFunction_t any[3];
+    explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
+        any[0] = d->kernel("attention_paged_any", "attn_paged_any_f16");
+        any[1] = d->kernel("attention_paged_any", "attn_paged_any_bf16");
+        any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
+    }
+};
+
+namespace {
+
+struct AttnPagedMeta : BatchMeta {
+    uint64_t dt;
+    size_t nh, nt, dh;
+};
+AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
+    expect_rank(a.q_layout, "q", 3);
+    expect_rank(a.o_layout, "o", 3);
+    AttnPagedMeta m;
+    static_cast<BatchMeta &>(m) = batch_meta(a.k_cache_layout, a.v_cache_layout, a.page_table_layout, a.q_start_layout, a.kv_len_layout);
+    m.dt = type_distinct({a.q_layout.dt, a.k_cache_layout.dt, a.v_cache_layout.dt, a.o_layout.dt});
+    expect_element_type(m.dt);
+    m.nh = dim_distinct({a.q_layout.shape[0], a.o_layout.shape[0]});
+    m.nt = dim_distinct({a.q_layout.shape[1], a.o_layout.shape[1]});
+    m.dh = dim_distinct({a.q_layout.shape[2], a.o_layout.shape[2], a.k_cache_layout.shape[3], a.v_cache_layout.shape[3]});
+    if (a.mask != OPHIP_MASK_NONE && a.mask != OPHIP_MASK_CAUSAL) throw args_not_support("unknown mask");
+    if (!is_dyn(m.nh) && !is_dyn(m.nkvh) && (m.nkvh == 0 ? m.nh != 0 : m.nh % m.nkvh != 0)) throw shape_mismatch("nh must be a multiple of nkvh");
+    if (!is_dyn(m.dh) && m.dh > MAX_HEAD) throw shape_not_support("head dimension too large");
+    return m;
+}
+
+void attention_paged_launch(const ophip_attention_paged *op, const ophip_attention_paged_args &a, void *workspace, size_t workspace_len,
+                            const ophip_queue_alloc *qa) {
+    const AttnPagedMeta m = attention_paged_meta(a);
+    const size_t nh = static_of(m.nh), nt = static_of(m.nt), dh = static_of(m.dh), nkvh = static_of(m.nkvh), nseq = static_of(m.nseq);
+    const float scale = static_of(a.scale);
+    if (std::isnan(scale) || std::isinf(scale)) throw args_not_support("scale must be a number");
+    expect_strides(a.q_layout, "q");
+    expect_strides(a.o_layout, "o");
+    expect_strides(a.k_cache_layout, "k_cache");
+    expect_strides(a.v_cache_layout, "v_cache");
+    (void)static_of(m.cols), (void)static_of(m.npages), (void)static_of(m.page);
+    if (nh == 0 || nt == 0 || dh == 0 || nseq == 0) return;
+    AttnPagedParams p{};
+    p.b = batch_params(m, nt, a.page_table_layout, a.page_table_base, a.q_start_layout, a.q_start_base, a.kv_len_layout, a.kv_len_base);
+    if (nh > MAX_INDEX / nt) throw shape_not_support("too many rows");
+    if (!a.q_base || !a.o_base || (p.b.cols && (!a.k_cache_base || !a.v_cache_base))) throw args_not_support("null base address");
+    // a workgroup writes rows of o while others still read: o lies apart from what is read, or is q itself, row by row
+    if (!same_view(a.o_layout, a.o_base, a.q_layout, a.q_base) && !apart(a.o_layout, a.o_base, a.q_layout, a.q_base))
+        throw args_not_support("o overlaps q");
+    if (!apart(a.o_layout, a.o_base, a.k_cache_layout, a.k_cache_base) || !apart(a.o_layout, a.o_base, a.v_cache_layout, a.v_cache_base))
+        throw args_not_support("o overlaps the cache");
+    p.q = a.q_base, p.o = a.o_base, p.k = a.k_cache_base, p.v = a.v_cache_base;
+    const ptrdiff_t *s = a.q_layout.strides;
+    p.q_sh = s[0], p.q_st = s[1], p.q_sd = s[2];
+    s = a.o_layout.strides;
+    p.o_sh = s[0], p.o_st = s[1], p.o_sd = s[2];
+    s = a.k_cache_layout.strides;
+    p.k_sp = s[0], p.k_sh = s[1], p.k_sr = s[2], p.k_sd = s[3];
+    s = a.v_cache_layout.strides;
+    p.v_sp = s[0], p.v_sh = s[1], p.v_sr = s[2], p.v_sd = s[3];
+    p.group = make_fastdiv((uint32_t)(nh / nkvh));
+    p.nkvh = (uint32_t)nkvh, p.dh = (uint32_t)dh, p.causal = a.mask == OPHIP_MASK_CAUSAL;
+    p.scale = scale;
+    op->dev->make_current();
+    launch(op->any[type_index(m.dt)], Dim3{(unsigned)(nt * nh)}, Dim3{256}, 0, stream_of(qa), p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ophip_attention_paged_create(ophip_device *dev, ophip_attention_paged **out) {
+    return guard([&] {
+        if (!dev || !out) throw args_not_support("null argument");
+        *out = new ophip_attention_paged(dev);
+    });
+}
+void ophip_attention_paged_destroy(ophip_attention_paged *op) { delete op; }
+
+int ophip_attention_paged_scheme(ophip_attention_paged *op, const ophip_attention_paged_args *args, size_t max_ws, size_t *ws) {
+    return guard([&] {
+        if (ws) *ws = 0;
+        if (!args) throw args_not_support("null argument");
+        (void)attention_paged_meta(*args);
+    });
+}
+
+int ophip_attention_paged_launch(const ophip_attention_paged *op, const ophip_attention_paged_args *args, void *workspace, size_t workspace_len,
+                                 const ophip_queue_alloc *qa) {
+    return guard([&] {
+        if (!op || !args) throw args_not_support("null argument");
+        attention_paged_launch(op, *args, workspace, workspace_len, qa);
+    });
+}
+
+}  // extern "C"
+
+// ============================================================== kv_append_paged ===
+
+struct ophip_kv_append_paged : OpBase {
+    hipFunction_t vec[3], pairs[3];
+    explicit ophip_kv_append_paged(ophip_device *d) : OpBase(d) {
+        static const char *tag[3] = {"f16", "bf16", "f32"};
+        for (int t = 0; t < 3; ++t) {
+            vec[t] = d->kernel("kv_append_paged", (std::string("kv_append_") + tag[t] + "_vec").c_str());
+            pairs[t] = d->kernel("kv_append_paged", (std::string("kv_append_") + tag[t] + "_pairs").c_str());
+        }
+    }
+};
+
+namespace {
+
+struct KvAppendMeta : BatchMeta {
+    uint64_t dt;
+    size_t nt, dh;
+};
+KvAppendMeta kv_append_paged_meta(const ophip_kv_append_paged_args &a) {
+    expect_rank(a.k_layout, "k", 3);
+    expect_rank(a.v_layout, "v", 3);
+    expect_rank(a.p_layout, "p", 1);
+    expect_position_type(a.p_layout.dt);
+    KvAppendMeta m;
+    static_cast<BatchMeta &>(m) = batch_meta(a.k_cache_layout, a.v_cache_layout, a.page_table_layout, a.q_start_layout, a.kv_len_layout);
+    m.dt = type_distinct({a.k_layout.dt, a.v_layout.dt, a.k_cache_layout.dt, a.v_cache_layout.dt});
+    expect_element_type(m.dt);
+    m.nkvh = dim_distinct({m.nkvh, a.k_layout.shape[0], a.v_layout.shape[0]});
+    m.nt = dim_distinct({a.k_layout.shape[1], a.v_layout.shape[1], a.p_layout.shape[0]});
+    m.dh = dim_distinct({a.k_layout.shape[2], a.v_layout.shape[2], a.k_cache_layout.shape[3], a.v_cache_layout.shape[3]});
+    if (!is_dyn(m.dh) && m.dh > MAX_HEAD) throw shape_not_support("head dimension too large");
+    return m;
+}
+
+void kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_append_paged_args &a, const ophip_queue_alloc *qa) {
+    const KvAppendMeta m = kv_append_paged_meta(a);
+    const size_t nt = static_of(m.nt), dh = static_of(m.dh), nkvh = static_of(m.nkvh), nseq = static_of(m.nseq);
+    KvAppendPagedParams p{};
+    p.rotate = rotation(a.theta, dh, &p.freq_step);
+    expect_strides(a.k_layout, "k");
+    expect_strides(a.v_layout, "v");
+    expect_strides(a.p_layout, "p");
+    expect_strides(a.k_cache_layout, "k_cache");
+    expect_strides(a.v_cache_layout, "v_cache");
+    (void)static_of(m.cols), (void)static_of(m.npages), (void)static_of(m.page);
+    if (nt == 0 || dh == 0 || nkvh == 0 || nseq == 0) return;
+    p.b = batch_params(m, nt, a.page_table_layout, a.page_table_base, a.q_start_layout, a.q_start_base, a.kv_len_layout, a.kv_len_base);
+    if (p.b.cols == 0) return;  // no place for any key
+    if (nkvh > MAX_INDEX / MAX_HEAD) throw shape_not_support("too many heads");
+    if (!a.k_base || !a.v_base || !a.k_cache_base || !a.v_cache_base || (p.rotate && !a.p_base)) throw args_not_support("null base address");
+    // a workgroup writes the cache while others still read k and v
+    const struct {
+        const ophip_tensor_layout &l;
+        const void *base;
+    } from[2] = {{a.k_layout, a.k_base}, {a.v_layout, a.v_base}};
+    for (const auto &f : from)
+        if (!apart(f.l, f.base, a.k_cache_layout, a.k_cache_base) || !apart(f.l, f.base, a.v_cache_layout, a.v_cache_base))
+            throw args_not_support("k or v overlaps the cache");
+    p.k = a.k_base, p.v = a.v_base, p.pos = a.p_base, p.k_cache = a.k_cache_base, p.v_cache = a.v_cache_base;
+    const ptrdiff_t *s = a.k_layout.strides;
+    p.k_sh = s[0], p.k_st = s[1], p.k_sd = s[2];
+    s = a.v_layout.strides;
+    p.v_sh = s[0], p.v_st = s[1], p.v_sd = s[2];
+    s = a.k_cache_layout.strides;
+    p.kc_sp = s[0], p.kc_sh = s[1], p.kc_sr = s[2], p.kc_sd = s[3];
+    s = a.v_cache_layout.strides;
+    p.vc_sp = s[0], p.vc_sh = s[1], p.vc_sr = s[2], p.vc_sd = s[3];
+    p.p_step = a.p_layout.strides[0];
+    p.pos_is_u64 = ophip_dtype_nbytes(a.p_layout.dt) == 8;
+    p.nkvh = (uint32_t)nkvh, p.dh = (uint32_t)dh;
+    const bool vec = dh * ophip_dtype_nbytes(m.dt) % 16 == 0 && vector_rows(a.k_layout, a.k_base) && vector_rows(a.v_layout, a.v_base) &&
+                     vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base);
+    op->dev->make_current();
+    launch((vec ? op->vec : op->pairs)[type_index(m.dt)], Dim3{(unsigned)nt}, Dim3{256}, p.rotate ? dh / 2 * 8 : 0, stream_of(qa), p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ophip_kv_append_paged_create(ophip_device *dev, ophip_kv_append_paged **out) {
+    return guard([&] {
+        if (!dev || !out) throw args_not_support("null argument");
+        *out = new ophip_kv_append_paged(dev);
+    });
+}
+void ophip_kv_append_paged_destroy(ophip_kv_append_paged *op) { delete op; }
+
+int ophip_kv_append_paged_scheme(ophip_kv_append_paged *, const ophip_kv_append_paged_args *args, size_t, size_t *ws) {
+    return guard([&] {
+        if (ws) *ws = 0;
+        if (!args) throw args_not_support("null argument");
+        (void)kv_append_paged_meta(*args);
+    });
+}
+
+int ophip_kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_append_paged_args *args, void *, size_t, const ophip_queue_alloc *qa) {
+    return guard([&] {
+        if (!op || !args) throw args_not_support("null argument");
+        kv_append_paged_launch(op, *args, qa);
+    });
+}
+
+}  // extern "C"
+
+// ================================================================= qk_norm_rope ===
+
+struct ophip_qk_norm_rope : OpBase {
+    hipFunction_t vec[3][4], pairs[3];  // vec: rows of 8, 16, 32, 64 lanes
+    explicit ophip_qk_norm_rope(ophip_device *d) : OpBase(d) {
+        static const char *tag[3] = {"f16", "bf16", "f32"}, *lanes[4] = {"_l8", "_l16", "_l32", "_l64"};
+        for (int t = 0; t < 3; ++t) {
+            const std::string name = std::string("qk_norm_rope_") + tag[t];
+            for (int l = 0; l < 4; ++l) vec[t][l] = d->kernel("qk_norm_rope", (name + lanes[l]).c_str());
+            pairs[t] = d->kernel("qk_norm_rope", (name + "_pairs").c_str());
+        }
+    }
+};
+
+namespace {
+
+struct QkNormRopeMeta {
+    uint64_t dt, dt_w;
+    size_t nt, nh, nkh, dh;
+};
+QkNormRopeMeta qk_norm_rope_meta(const ophip_qk_norm_rope_args &a) {
+    expect_rank(a.qy_layout, "qy", 3);
+    expect_rank(a.q_layout, "q", 3);
+    expect_rank(a.qw_layout, "qw", 1);
+    expect_rank(a.ky_layout, "ky", 3);
+    expect_rank(a.k_layout, "k", 3);
+    expect_rank(a.kw_layout, "kw", 1);
+    expect_rank(a.p_layout, "p", 1);
+    QkNormRopeMeta m;
+    m.dt = type_distinct({a.qy_layout.dt, a.q_layout.dt, a.ky_layout.dt, a.k_layout.dt});
+    m.dt_w = type_distinct({a.qw_layout.dt, a.kw_layout.dt});
+    expect_element_type(m.dt);
+    if (m.dt_w != m.dt && m.dt_w != OPHIP_DT_F32) throw type_not_support("the weights have the rows' type or f32");
+    expect_position_type(a.p_layout.dt);
+    m.nt = dim_distinct({a.qy_layout.shape[0], a.q_layout.shape[0], a.ky_layout.shape[0], a.k_layout.shape[0], a.p_layout.shape[0]});
+    m.nh = dim_distinct({a.qy_layout.shape[1], a.q_layout.shape[1]});
+    m.nkh = dim_distinct({a.ky_layout.shape[1], a.k_layout.shape[1]});
+    m.dh = dim_distinct({a.qy_layout.shape[2], a.q_layout.shape[2], a.ky_layout.shape[2], a.k_layout.shape[2], a.qw_layout.shape[0], a.kw_layout.shape[0]});
+    if (!is_dyn(m.dh) && (m.dh > MAX_HEAD || m.dh % 2)) throw shape_not_support("head dimension odd or too large");
+    return m;
+}
+
+void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_args &a, const ophip_queue_alloc *qa) {
+    const QkNormRopeMeta m = qk_norm_rope_meta(a);
+    const size_t nt = static_of(m.nt), nh = static_of(m.nh), nkh = static_of(m.nkh), dh = static_of(m.dh), heads = nh + nkh;
+    QkNormRopeParams p{};
+    p.rotate = rotation(a.theta, dh, &p.freq_step);
+    p.epsilon = static_of(a.epsilon);
+    const ptrdiff_t unit = (ptrdiff_t)ophip_dtype_nbytes(m.dt), wunit = (ptrdiff_t)ophip_dtype_nbytes(m.dt_w);
+    expect_strides(a.p_layout, "p");
+    const struct {
+        const ophip_tensor_layout &y, &x, &w;
+        void *y_base;
+        const void *x_base, *w_base;
+        size_t nh;
+    } half[2] = {{a.qy_layout, a.q_layout, a.qw_layout, a.qy_base, a.q_base, a.qw_base, nh}, {a.ky_layout, a.k_layout, a.kw_layout, a.ky_base, a.k_base, a.kw_base, nkh}};
+    bool vec = dh * unit % 16 == 0;
+    for (int i = 0; i < 2; ++i) {
+        expect_strides(half[i].y, "y");
+        expect_strides(half[i].x, "x");
+        expect_strides(half[i].w, "w");
+        if (dh && (half[i].y.strides[2] != unit || half[i].x.strides[2] != unit || half[i].w.strides[0] != wunit))
+            throw strides_not_support("qk_norm_rope needs a contiguous head dimension");
+        p.x[i] = half[i].x_base, p.y[i] = half[i].y_base, p.w[i] = half[i].w_base;
+        p.x_st[i] = half[i].x.strides[0], p.x_sh[i] = half[i].x.strides[1], p.y_st[i] = half[i].y.strides[0], p.y_sh[i] = half[i].y.strides[1];
+        p.nh[i] = (uint32_t)half[i].nh;
+    }
+    if (nt == 0 || heads == 0 || dh == 0) return;
+    if (nt > MAX_INDEX || nh > 0xffffu || nkh > 0xffffu) throw shape_not_support("too many tokens or heads");
+    for (int i = 0; i < 2; ++i) {
+        const auto &h = half[i];
+        if (h.nh == 0) continue;
+        if (!h.y_base || !h.x_base || !h.w_base) throw args_not_support("null base address");
+        if (!same_view(h.y, h.y_base, h.x, h.x_base) && !apart(h.y, h.y_base, h.x, h.x_base)) throw args_not_support("y overlaps its x");
+        vec = vec && vector_rows(h.y, h.y_base) && vector_rows(h.x, h.x_base);
+    }
+    if (p.rotate && !a.p_base) throw args_not_support("null base address");
+    p.pos = a.p_base;
+    p.p_step = a.p_layout.strides[0];
+    p.pos_is_u64 = ophip_dtype_nbytes(a.p_layout.dt) == 8;
+    p.nt = (uint32_t)nt, p.dh = (uint32_t)dh;
+    p.w_is_f32 = m.dt_w == OPHIP_DT_F32;
+    const size_t vectors = dh * unit / 16;
+    vec = vec && vectors <= 64;
+    const int li = vectors <= 8 ? 0 : vectors <= 16 ? 1 : vectors <= 32 ? 2 : 3;
+    // few tokens: a token's heads over several workgroups, down to one row for each group of lanes
+    const size_t rows = vec ? 32u >> li : 4;
+    const size_t by = std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt));
+    p.heads_per_block = (uint32_t)((heads + by - 1) / by);
+    op->dev->make_current();
+    const int t = type_index(m.dt);
+    launch(vec ? op->vec[t][li] : op->pairs[t], Dim3{(unsigned)nt, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block)}, Dim3{256},
+           p.rotate ? dh / 2 * 8 : 0, stream_of(qa), p);
+}
+
+}  // namespace
+
+extern "C" {
+
+int ophip_qk_norm_rope_create(ophip_device *dev, ophip_qk_norm_rope **out) {
+    return guard([&] {
+        if (!dev || !out) throw args_not_support("null argument");
+        *out = new ophip_qk_norm_rope(dev);
+    });
+}
+void ophip_qk_norm_rope_destroy(ophip_qk_norm_rope *op) { delete op; }
+
+int ophip_qk_norm_rope_scheme(ophip_qk_norm_rope *, const ophip_qk_norm_rope_args *args, size_t, size_t *ws) {
+    return guard([&] {
+        if (ws) *ws = 0;
+        if (!args) throw args_not_support("null argument");
+        (void)qk_norm_rope_meta(*args);
+    });
+}
+
+int ophip_qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_args *args, void *, size_t, const ophip_queue_alloc *qa) {
+    return guard([&] {
+        if (!op || !args) throw args_not_support("null argument");
+        qk_norm_rope_launch(op, *args, qa);
+    });
+}
+
+}  // extern "C"

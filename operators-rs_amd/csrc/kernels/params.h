@@ -267,3 +267,52 @@ struct AddRowsParams {
     uint32_t idx_is_u64;
     uint32_t _pad;
 };
+
+// A packed batch of sequences over a paged cache, shared by attention_paged and kv_append_paged.  Strides in bytes.
+struct PagedBatch {
+    const void *table;            // u32 page numbers, one row per sequence
+    const void *q_start, *kv_len;  // u32: nseq + 1 and nseq values
+    int64_t t_row, t_col, s_step, l_step;
+    uint32_t nseq, nt, cols, npages;
+    FastDivU32 page;  // tokens per page
+};
+
+// attention over a paged cache (attention_paged.hip, attention_paged_any.hip).  Strides in bytes.
+struct AttnPagedParams {
+    struct PagedBatch b;
+    const void *q;
+    void *o;
+    const void *k, *v;
+    void *work;  // partial results of key ranges, when a tile's keys are split over workgroups (layout: attention_paged.hip)
+    int64_t q_sh, q_st, q_sd, o_sh, o_st, o_sd;
+    int64_t k_sp, k_sh, k_sr, k_sd, v_sp, v_sh, v_sr, v_sd;  // page, head, row in page, element
+    FastDivU32 group;  // query heads per kv head
+    uint32_t nkvh, dh, causal;
+    uint32_t slots;     // key ranges the work area holds, and the number that the tiles are split into together; 0: no splitting
+    uint32_t min_steps;  // a range has at least this many steps of 32 keys
+    float scale;
+};
+
+// k, v appended to a paged cache (kv_append_paged.hip).  Strides in bytes.
+struct KvAppendPagedParams {
+    struct PagedBatch b;
+    const void *k, *v, *pos;
+    void *k_cache, *v_cache;
+    int64_t k_sh, k_st, k_sd, v_sh, v_st, v_sd, p_step;
+    int64_t kc_sp, kc_sh, kc_sr, kc_sd, vc_sp, vc_sh, vc_sr, vc_sd;
+    uint32_t nkvh, dh, pos_is_u64, rotate;
+    double freq_step;  // log2(theta) / (dh / 2)
+};
+
+// rms_norm of every query and key head, then rope, in one pass (qk_norm_rope.hip).  Strides in bytes.
+struct QkNormRopeParams {
+    const void *x[2], *w[2], *pos;  // [0] the queries, [1] the keys
+    void *y[2];
+    int64_t x_st[2], x_sh[2], y_st[2], y_sh[2], p_step;
+    uint32_t nt, nh[2], dh;
+    uint32_t heads_per_block;  // of the nh[0] + nh[1] heads of a token
+    uint32_t pos_is_u64, rotate, w_is_f32;
+    float epsilon;
+    uint32_t _pad;
+    double freq_step;  // log2(theta) / (dh / 2)
+};

@@ -169,6 +169,28 @@ class _AttnKVCachedArgs(ctypes.Structure):
                 ("mask", ctypes.c_uint8), ("pos", ctypes.c_size_t)]
 
 
+class _AttentionPagedArgs(ctypes.Structure):
+    _fields_ = [("q_layout", _Layout), ("q_base", ctypes.c_void_p), ("k_cache_layout", _Layout), ("k_cache_base", ctypes.c_void_p),
+                ("v_cache_layout", _Layout), ("v_cache_base", ctypes.c_void_p), ("o_layout", _Layout), ("o_base", ctypes.c_void_p),
+                ("page_table_layout", _Layout), ("page_table_base", ctypes.c_void_p), ("q_start_layout", _Layout), ("q_start_base", ctypes.c_void_p),
+                ("kv_len_layout", _Layout), ("kv_len_base", ctypes.c_void_p), ("mask", ctypes.c_uint8), ("scale", ctypes.c_float)]
+
+
+class _KvAppendPagedArgs(ctypes.Structure):
+    _fields_ = [("k_layout", _Layout), ("k_base", ctypes.c_void_p), ("v_layout", _Layout), ("v_base", ctypes.c_void_p),
+                ("p_layout", _Layout), ("p_base", ctypes.c_void_p), ("k_cache_layout", _Layout), ("k_cache_base", ctypes.c_void_p),
+                ("v_cache_layout", _Layout), ("v_cache_base", ctypes.c_void_p), ("page_table_layout", _Layout), ("page_table_base", ctypes.c_void_p),
+                ("q_start_layout", _Layout), ("q_start_base", ctypes.c_void_p), ("kv_len_layout", _Layout), ("kv_len_base", ctypes.c_void_p),
+                ("theta", ctypes.c_float)]
+
+
+class _QkNormRopeArgs(ctypes.Structure):
+    _fields_ = [("qy_layout", _Layout), ("qy_base", ctypes.c_void_p), ("q_layout", _Layout), ("q_base", ctypes.c_void_p),
+                ("qw_layout", _Layout), ("qw_base", ctypes.c_void_p), ("ky_layout", _Layout), ("ky_base", ctypes.c_void_p),
+                ("k_layout", _Layout), ("k_base", ctypes.c_void_p), ("kw_layout", _Layout), ("kw_base", ctypes.c_void_p),
+                ("p_layout", _Layout), ("p_base", ctypes.c_void_p), ("epsilon", ctypes.c_float), ("theta", ctypes.c_float)]
+
+
 class _LayerNormArgs(ctypes.Structure):
     _fields_ = [("y_layout", _Layout), ("y_base", ctypes.c_void_p), ("x_layout", _Layout),
                 ("x_base", ctypes.c_void_p), ("scale_layout", _Layout), ("scale_base", ctypes.c_void_p),
@@ -226,6 +248,12 @@ EXPORTS = [
     "ophip_attention_create", "ophip_attention_scheme", "ophip_attention_launch", "ophip_attention_destroy",
     "ophip_attention_kv_cached_create", "ophip_attention_kv_cached_scheme", "ophip_attention_kv_cached_launch",
     "ophip_attention_kv_cached_destroy",
+    "ophip_attention_paged_create", "ophip_attention_paged_scheme", "ophip_attention_paged_launch",
+    "ophip_attention_paged_destroy",
+    "ophip_kv_append_paged_create", "ophip_kv_append_paged_scheme", "ophip_kv_append_paged_launch",
+    "ophip_kv_append_paged_destroy",
+    "ophip_qk_norm_rope_create", "ophip_qk_norm_rope_scheme", "ophip_qk_norm_rope_launch",
+    "ophip_qk_norm_rope_destroy",
     "ophip_layer_norm_create", "ophip_layer_norm_scheme", "ophip_layer_norm_launch", "ophip_layer_norm_destroy",
     "ophip_gelu_create", "ophip_gelu_scheme", "ophip_gelu_launch", "ophip_gelu_destroy",
     "ophip_add_create", "ophip_add_scheme", "ophip_add_launch", "ophip_add_destroy", "ophip_add_plan",
@@ -330,6 +358,16 @@ class Stream:
         if self.handle is not None:
             lib().ophip_stream_destroy(self.gpu.handle, self.handle)
             self.handle = None
+
+
+class ExternalStream:
+    """A stream made elsewhere (a hipStream_t as an integer; 0: the default stream) as a queue for launches.  It stays its
+    maker's: nothing here destroys it."""
+
+    def __init__(self, gpu, handle):
+        self.gpu, self.handle = gpu, ctypes.c_void_p(handle or None)
+        self.queue_alloc = _QueueAlloc()
+        _check(lib().ophip_queue_alloc_from_stream(gpu.handle, self.handle, ctypes.byref(self.queue_alloc)))
 
 
 class Graph:
@@ -687,6 +725,53 @@ class AttnKVCachedArgs:
                                  DYN_USIZE if self.pos is None else self.pos)
 
 
+class AttentionPagedArgs:
+    """attention over a paged cache; the layouts are described in include/ophip.h"""
+
+    def __init__(self, q_layout, q_base, k_cache_layout, k_cache_base, v_cache_layout, v_cache_base, o_layout,
+                 o_base, page_table_layout, page_table_base, q_start_layout, q_start_base, kv_len_layout,
+                 kv_len_base, mask, scale):
+        self.__dict__.update(locals())
+
+    def c(self):
+        return _AttentionPagedArgs(self.q_layout.c(), _p(self.q_base), self.k_cache_layout.c(),
+                                    _p(self.k_cache_base), self.v_cache_layout.c(), _p(self.v_cache_base),
+                                    self.o_layout.c(), _p(self.o_base), self.page_table_layout.c(),
+                                    _p(self.page_table_base), self.q_start_layout.c(), _p(self.q_start_base),
+                                    self.kv_len_layout.c(), _p(self.kv_len_base), self.mask, self.scale)
+
+
+class KvAppendPagedArgs:
+    """k and v into a paged cache, k rotated on the way (theta = 0: not)"""
+
+    def __init__(self, k_layout, k_base, v_layout, v_base, p_layout, p_base, k_cache_layout, k_cache_base,
+                 v_cache_layout, v_cache_base, page_table_layout, page_table_base, q_start_layout,
+                 q_start_base, kv_len_layout, kv_len_base, theta):
+        self.__dict__.update(locals())
+
+    def c(self):
+        return _KvAppendPagedArgs(self.k_layout.c(), _p(self.k_base), self.v_layout.c(), _p(self.v_base),
+                                   self.p_layout.c(), _p(self.p_base), self.k_cache_layout.c(),
+                                   _p(self.k_cache_base), self.v_cache_layout.c(), _p(self.v_cache_base),
+                                   self.page_table_layout.c(), _p(self.page_table_base),
+                                   self.q_start_layout.c(), _p(self.q_start_base), self.kv_len_layout.c(),
+                                   _p(self.kv_len_base), self.theta)
+
+
+class QkNormRopeArgs:
+    """rms_norm of every query and key head, then rope (theta = 0: the norms alone)"""
+
+    def __init__(self, qy_layout, qy_base, q_layout, q_base, qw_layout, qw_base, ky_layout, ky_base, k_layout,
+                 k_base, kw_layout, kw_base, p_layout, p_base, epsilon, theta):
+        self.__dict__.update(locals())
+
+    def c(self):
+        return _QkNormRopeArgs(self.qy_layout.c(), _p(self.qy_base), self.q_layout.c(), _p(self.q_base),
+                                self.qw_layout.c(), _p(self.qw_base), self.ky_layout.c(), _p(self.ky_base),
+                                self.k_layout.c(), _p(self.k_base), self.kw_layout.c(), _p(self.kw_base),
+                                self.p_layout.c(), _p(self.p_base), self.epsilon, self.theta)
+
+
 class LayerNormArgs:
     """layer_norm/args.rs:7-17"""
 
@@ -826,6 +911,18 @@ class Attention(_Operator):
 
 class AttnKVCached(_Operator):
     NAME = "attention_kv_cached"
+
+
+class AttentionPaged(_Operator):
+    NAME = "attention_paged"
+
+
+class KvAppendPaged(_Operator):
+    NAME = "kv_append_paged"
+
+
+class QkNormRope(_Operator):
+    NAME = "qk_norm_rope"
 
 
 class RandomSample(_Operator):

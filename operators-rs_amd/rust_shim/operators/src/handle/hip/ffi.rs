@@ -131,6 +131,64 @@ pub struct ophip_mat_mul_args {
 }
 
 #[repr(C)]
+pub struct ophip_attention_paged_args {
+    pub q_layout: ophip_tensor_layout,
+    pub q_base: *const c_void,
+    pub k_cache_layout: ophip_tensor_layout,
+    pub k_cache_base: *const c_void,
+    pub v_cache_layout: ophip_tensor_layout,
+    pub v_cache_base: *const c_void,
+    pub o_layout: ophip_tensor_layout,
+    pub o_base: *mut c_void,
+    pub page_table_layout: ophip_tensor_layout,
+    pub page_table_base: *const c_void,
+    pub q_start_layout: ophip_tensor_layout,
+    pub q_start_base: *const c_void,
+    pub kv_len_layout: ophip_tensor_layout,
+    pub kv_len_base: *const c_void,
+    pub mask: u8,
+    pub scale: f32,
+}
+#[repr(C)]
+pub struct ophip_kv_append_paged_args {
+    pub k_layout: ophip_tensor_layout,
+    pub k_base: *const c_void,
+    pub v_layout: ophip_tensor_layout,
+    pub v_base: *const c_void,
+    pub p_layout: ophip_tensor_layout,
+    pub p_base: *const c_void,
+    pub k_cache_layout: ophip_tensor_layout,
+    pub k_cache_base: *mut c_void,
+    pub v_cache_layout: ophip_tensor_layout,
+    pub v_cache_base: *mut c_void,
+    pub page_table_layout: ophip_tensor_layout,
+    pub page_table_base: *const c_void,
+    pub q_start_layout: ophip_tensor_layout,
+    pub q_start_base: *const c_void,
+    pub kv_len_layout: ophip_tensor_layout,
+    pub kv_len_base: *const c_void,
+    pub theta: f32,
+}
+#[repr(C)]
+pub struct ophip_qk_norm_rope_args {
+    pub qy_layout: ophip_tensor_layout,
+    pub qy_base: *mut c_void,
+    pub q_layout: ophip_tensor_layout,
+    pub q_base: *const c_void,
+    pub qw_layout: ophip_tensor_layout,
+    pub qw_base: *const c_void,
+    pub ky_layout: ophip_tensor_layout,
+    pub ky_base: *mut c_void,
+    pub k_layout: ophip_tensor_layout,
+    pub k_base: *const c_void,
+    pub kw_layout: ophip_tensor_layout,
+    pub kw_base: *const c_void,
+    pub p_layout: ophip_tensor_layout,
+    pub p_base: *const c_void,
+    pub epsilon: f32,
+    pub theta: f32,
+}
+#[repr(C)]
 pub struct ophip_layer_norm_args {
     pub y_layout: ophip_tensor_layout,
     pub y_base: *mut c_void,
@@ -197,6 +255,9 @@ verbs! {
     ophip_swiglu, ophip_swiglu_args, ophip_swiglu_create, ophip_swiglu_scheme, ophip_swiglu_launch, ophip_swiglu_destroy;
     ophip_random_sample, ophip_random_sample_args, ophip_random_sample_create, ophip_random_sample_scheme, ophip_random_sample_launch, ophip_random_sample_destroy;
     ophip_mat_mul, ophip_mat_mul_args, ophip_mat_mul_create, ophip_mat_mul_scheme, ophip_mat_mul_launch, ophip_mat_mul_destroy;
+    ophip_attention_paged, ophip_attention_paged_args, ophip_attention_paged_create, ophip_attention_paged_scheme, ophip_attention_paged_launch, ophip_attention_paged_destroy;
+    ophip_kv_append_paged, ophip_kv_append_paged_args, ophip_kv_append_paged_create, ophip_kv_append_paged_scheme, ophip_kv_append_paged_launch, ophip_kv_append_paged_destroy;
+    ophip_qk_norm_rope, ophip_qk_norm_rope_args, ophip_qk_norm_rope_create, ophip_qk_norm_rope_scheme, ophip_qk_norm_rope_launch, ophip_qk_norm_rope_destroy;
     ophip_layer_norm, ophip_layer_norm_args, ophip_layer_norm_create, ophip_layer_norm_scheme, ophip_layer_norm_launch, ophip_layer_norm_destroy;
     ophip_gelu, ophip_gelu_args, ophip_gelu_create, ophip_gelu_scheme, ophip_gelu_launch, ophip_gelu_destroy;
     ophip_add, ophip_add_args, ophip_add_create, ophip_add_scheme, ophip_add_launch, ophip_add_destroy;

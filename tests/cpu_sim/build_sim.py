@@ -25,7 +25,7 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 CSRC = os.path.join(ROOT, "operators-rs_amd", "csrc")
 KERNELS = os.path.join(CSRC, "kernels")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
-HOST_OBJECTS = ["handle", "ops", "random_sample", "mat_mul", "attention", "ops_more", "conv", "static_scratch"]
+HOST_OBJECTS = ["handle", "ops", "random_sample", "mat_mul", "attention", "ops_more", "conv", "paged", "static_scratch"]
 DEVICE_FLAGS = ["-std=c++20", "-O1", "-fPIC", "-x", "c++", "-I", HERE, "-I", KERNELS, "-DOPHIP_CPU_SIM=1", "-Wno-unused-value",
                 "-Wno-pass-failed", "-Wno-unknown-attributes"]
 

@@ -68,6 +68,10 @@ inline uint32_t __umulhi(uint32_t a, uint32_t b) { return (uint32_t)(((uint64_t)
 inline int __ffsll(long long v) { return __builtin_ffsll(v); }
 inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 inline float rsqrtf(float x) { return 1.0f / sqrtf(x); }
+inline void sincospif(float x, float *s, float *c) {
+    *s = (float)sin(M_PI * (double)x);
+    *c = (float)cos(M_PI * (double)x);
+}
 inline double rsqrt(double x) { return 1.0 / sqrt(x); }
 #define __builtin_amdgcn_readfirstlane(x) (x)
 #define __builtin_amdgcn_sched_barrier(mask) ((void)0)

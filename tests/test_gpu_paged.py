@@ -1,0 +1,697 @@
+"""The operators over a paged cache (attention_paged, kv_append_paged, qk_norm_rope) against their definitions in 64 bits.
+
+Tolerances.  u = half a step of the type (bf16 2^-8, f16 2^-11, f32 2^-24), e = 2^-24.
+  * attention: the result is rounded once (u), the probabilities are rounded to the type before the second product (u, of
+    each term p v, so of sum p |v| / sum p =: A), and a score is a sum of dh products in f32 (at most (dh + 8) e of
+    S = scale * sum |q| |k|, which moves a probability by as much, in the numerator and in the sum); 2^-20 of A for the
+    exponentials and the sums over keys: |o - o64| <= (2 u + 2 (dh + 8) e S + 2^-20) A.
+  * rotation: one rounding (u), sine and cosine to 2^-22, products and their sum: u |y| + 2^-20 (|a| + |b|) for the pair.
+  * norm: a sum of dh squares ((dh / 2 + 8) e of the normalised row), then the rotation.
+f16 results below 2^-14 are rounded in steps of 2^-24: 2^-25 more.
+"""
+import ctypes
+
+import numpy as np
+import pytest
+
+import ophip
+from ophip import TensorLayout, dt
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f16": 2.0 ** -11, "bf16": 2.0 ** -8, "f32": 2.0 ** -24}
+CODE = {"f16": dt.F16, "bf16": dt.BF16, "f32": dt.F32}
+SIZE = {"f16": 2, "bf16": 2, "f32": 4}
+E = 2.0 ** -24
+
+
+def encode(x, kind):
+    """f64 values rounded to the type, as the bits that are uploaded."""
+    x = np.asarray(x, np.float32)
+    if kind == "f16":
+        return x.astype(np.float16)
+    if kind == "f32":
+        return x
+    b = np.ascontiguousarray(x).view(np.uint32)
+    r = ((b + 0x7FFF + ((b >> 16) & 1)) >> 16).astype(np.uint16)
+    return np.where(np.isnan(x), np.uint16(0x7FC0), r).astype(np.uint16)
+
+
+def decode(bits, kind):
+    if kind == "bf16":
+        return (bits.astype(np.uint32) << 16).view(np.float32).astype(np.float64)
+    return bits.astype(np.float64)
+
+
+def store(kind):
+    return {"f16": np.float16, "bf16": np.uint16, "f32": np.float32}[kind]
+
+
+def layout(view, kind):
+    return TensorLayout(CODE[kind], view.shape, view.strides)
+
+
+class Buffer:
+    """A host array and its copy on the device; `view(x)`: the layout and address of a numpy view of it."""
+
+    def __init__(self, gpu, array, kind=None):
+        self.gpu, self.host, self.kind = gpu, np.ascontiguousarray(array), kind
+        self.mem = gpu.from_host(self.host)
+
+    def view(self, x=None):
+        x = self.host if x is None else x
+        off = x.__array_interface__["data"][0] - self.host.__array_interface__["data"][0] if x.size else 0
+        code = CODE[self.kind] if self.kind else {np.dtype(np.uint32): dt.U32, np.dtype(np.int32): dt.I32, np.dtype(np.uint64): dt.U64, np.dtype(np.int64): dt.I64}[x.dtype]
+        return TensorLayout(code, x.shape, x.strides), self.mem.ptr + off
+
+    def back(self, stream):
+        return self.gpu.to_host(self.mem, self.host.dtype, self.host.size, stream=stream).reshape(self.host.shape)
+
+
+class Batch:
+    """A paged cache and a packed batch: lens = [(new tokens, keys)], `pad` tokens behind them."""
+
+    def __init__(self, gpu, rng, kind, nh, nkvh, dh, page, lens, pad=0, spare=2, junk=np.nan, token_major=False, head_gap=0):
+        self.kind, self.nh, self.nkvh, self.dh, self.page, self.lens = kind, nh, nkvh, dh, page, lens
+        self.start = np.concatenate([[0], np.cumsum([n for n, _ in lens])]).astype(np.uint32)
+        self.nt = int(self.start[-1]) + pad
+        used = [-(-l // page) for _, l in lens]
+        npages, cols = sum(used) + spare, max(1, max(used))
+        order = rng.permutation(npages)
+        table, at = np.full((len(lens), cols), 0xFFFFFFFF, np.uint32), 0
+        for s, c in enumerate(used):
+            table[s, :c] = order[at:at + c]
+            at += c
+        shape = (npages, page, nkvh, dh + head_gap) if token_major else (npages, nkvh, page, dh + head_gap)
+        cache = [np.full(shape, junk, np.float64) for _ in range(2)]
+        views = [(c.swapaxes(1, 2) if token_major else c)[..., :dh] for c in cache]
+        for s, (_, l) in enumerate(lens):
+            for j in range(l):
+                for v in views:
+                    v[table[s, j // page], :, j % page] = rng.standard_normal((nkvh, dh))
+        self.cache = [Buffer(gpu, encode(c, kind), kind) for c in cache]
+        self.cache_views = [(c.host.swapaxes(1, 2) if token_major else c.host)[..., :dh] for c in self.cache]
+        self.table, self.q_start = Buffer(gpu, table), Buffer(gpu, self.start)
+        self.kv_len = Buffer(gpu, np.array([l for _, l in lens], np.uint32))
+        self.q = Buffer(gpu, encode(rng.standard_normal((self.nt, nh, dh)) * 1.5, kind), kind)
+        self.o = Buffer(gpu, encode(np.full((self.nt, nh, dh), 0.125), kind), kind)
+
+    def batch_args(self):
+        return self.table.view() + self.q_start.view() + self.kv_len.view()
+
+    def cache_args(self):
+        return self.cache[0].view(self.cache_views[0]) + self.cache[1].view(self.cache_views[1])
+
+    def args(self, mask, scale=None):
+        scale = self.dh ** -0.5 if scale is None else scale
+        q, o = self.q.host.transpose(1, 0, 2), self.o.host.transpose(1, 0, 2)
+        return ophip.AttentionPagedArgs(*self.q.view(q), *self.cache_args(), *self.o.view(o), *self.batch_args(), mask, scale)
+
+    def keys(self, s, which, cache=None):
+        l = self.lens[s][1]
+        views = self.cache_views if cache is None else cache
+        rows = [views[which][self.table.host[s, j // self.page], :, j % self.page] for j in range(l)]
+        return decode(np.array(rows).reshape(l, self.nkvh, self.dh), self.kind)
+
+    def expected(self, mask, scale=None, q=None, cache=None):
+        """(o in 64 bits, tolerance); rows of no sequence as they were, tolerance 0."""
+        scale = float(np.float32(self.dh ** -0.5 if scale is None else scale))
+        q = decode(self.q.host, self.kind) if q is None else q
+        o, tol = decode(self.o.host, self.kind), np.zeros((self.nt, self.nh, self.dh))
+        u, group = HALF[self.kind], self.nh // self.nkvh
+        for s, (n, l) in enumerate(self.lens):
+            k, v = self.keys(s, 0, cache), self.keys(s, 1, cache)
+            for i in range(n):
+                t, keep = self.start[s] + i, min(l, max(0, l - n + i + 1)) if mask else l
+                for h in range(self.nh):
+                    if keep == 0:
+                        o[t, h], tol[t, h] = 0, 0
+                        continue
+                    kk, vv = k[:keep, h // group], v[:keep, h // group]
+                    x = kk @ q[t, h] * scale
+                    p = np.exp(x - x.max())
+                    p /= p.sum()
+                    o[t, h] = p @ vv
+                    big = (np.abs(kk) @ np.abs(q[t, h])).max() * abs(scale)
+                    tol[t, h] = (2 * u + 2 * (self.dh + 8) * E * big + 2.0 ** -20) * (p @ np.abs(vv)) + 2.0 ** -25
+        return o, tol
+
+
+def check(got, want, tol, what=""):
+    assert np.array_equal(np.isnan(got), np.isnan(want)), what
+    off = np.abs(got - want) - tol
+    assert (off <= 0).all(), "%s: %d of %d beyond their tolerance, worst by %g at %s" % (
+        what, (off > 0).sum(), off.size, off.max(), np.unravel_index(np.argmax(off), off.shape))
+
+
+def run(gpu, stream, args, op=None, workspace=True):
+    op = op or ophip.AttentionPaged(gpu)
+    need = op.scheme(args, 1 << 40)
+    ws = gpu.malloc(need) if need and workspace else None
+    op.launch(args, ws, stream)
+    stream.synchronize()
+    return ws
+
+
+def attend(gpu, stream, b, mask, **kw):
+    run(gpu, stream, b.args(mask, kw.pop("scale", None)), **kw)
+    return decode(b.o.back(stream), b.kind)
+
+
+SHAPES = [  # nh, nkvh, dh, page, lens
+    (4, 4, 64, 16, [(1, 1)]),
+    (4, 1, 64, 16, [(1, 33), (1, 16), (1, 0), (1, 300)]),
+    (8, 2, 128, 7, [(1, 5), (1, 129), (1, 640)]),
+    (7, 1, 128, 32, [(1, 1000)]),
+    (16, 1, 64, 1, [(1, 77), (1, 257)]),
+    (20, 1, 128, 24, [(1, 200), (2, 31)]),
+    (6, 3, 64, 24, [(5, 5), (0, 40), (3, 50), (9, 9)]),
+    (4, 4, 128, 64, [(70, 70), (3, 200)]),
+    (2, 2, 64, 128, [(130, 400)]),
+    (8, 2, 128, 16, [(33, 33), (65, 130), (1, 17)]),
+    (3, 1, 64, 256, [(150, 150)]),
+    (12, 4, 64, 100, [(40, 700), (1, 900), (2, 3)]),
+    (24, 1, 128, 48, [(11, 95)]),
+    (4, 2, 128, 16, [(10, 4), (6, 0), (3, 3)]),  # fewer keys than tokens: rows that see nothing
+    (2, 1, 40, 16, [(3, 50)]),                     # a head dimension of no matrix kernel
+    (2, 2, 8, 5, [(4, 21), (1, 7)]),
+    (1, 1, 1, 3, [(2, 9)]),
+]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("mask", [1, 0])
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%d-%d-%d-%d-%s" % (s[0], s[1], s[2], s[3], "_".join("%dof%d" % x for x in s[4])))
+def test_attention_paged(gpu, stream, shape, mask, kind):
+    rng = np.random.default_rng(7)
+    b = Batch(gpu, rng, kind, *shape[:4], shape[4], pad=3)
+    want, tol = b.expected(mask)
+    check(attend(gpu, stream, b, mask), want, tol)
+    assert np.array_equal(b.q.back(stream).view(np.uint8), b.q.host.view(np.uint8))  # q is read only
+    for c in b.cache:
+        assert np.array_equal(c.back(stream).view(np.uint8), c.host.view(np.uint8))
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("lens", [[(1, 3000)], [(1, 3000), (1, 10), (1, 700)], [(40, 2500)], [(16, 1500), (1, 5), (90, 90)]], ids=str)
+def test_attention_paged_keys_split_over_workgroups(gpu, stream, lens, kind):
+    """Few rows and many keys: a tile's keys go to several workgroups and are joined; with the workspace that scheme
+    reports, and with one from the queue's allocator."""
+    rng = np.random.default_rng(8)
+    b = Batch(gpu, rng, kind, 4, 1, 128, 32, lens)
+    want, tol = b.expected(1)
+    one = attend(gpu, stream, b, 1)
+    check(one, want, tol)
+    b.o.gpu.upload(b.o.mem, b.o.host)
+    two = attend(gpu, stream, b, 1, workspace=False)
+    assert np.array_equal(one, two)  # the same bits
+
+
+@pytest.mark.parametrize("shape", [(4, 2, 64, 16, [(1, 90), (1, 40)]), (4, 2, 128, 16, [(50, 90), (1, 40)])], ids=["few", "many"])
+@pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap", "fused_qkv", "o_over_q", "strided_batch"])
+def test_attention_paged_views(gpu, stream, form, shape):
+    """Caches with the tokens of a page in front of the heads, rows farther apart (on 16-byte boundaries and not), q a view of
+    a fused projection, o in place of q, and tables and lengths that are views themselves."""
+    rng = np.random.default_rng(9)
+    b = Batch(gpu, rng, "f16", *shape[:4], shape[4], pad=1, token_major=form == "token_major", head_gap={"head_gap": 8, "odd_gap": 3}.get(form, 0))
+    want, tol = b.expected(1)
+    scale, q, o = b.dh ** -0.5, b.q.host.transpose(1, 0, 2), b.o.host.transpose(1, 0, 2)
+    qa, oa, batch = b.q.view(q), b.o.view(o), b.batch_args()
+    if form == "fused_qkv":
+        wide = np.zeros((b.nt, (b.nh + 2 * b.nkvh) * b.dh), np.float16)
+        wide[:, :b.nh * b.dh] = b.q.host.reshape(b.nt, -1)
+        fused = Buffer(gpu, wide, "f16")
+        qa = fused.view(fused.host[:, :b.nh * b.dh].reshape(b.nt, b.nh, b.dh).transpose(1, 0, 2))
+    if form == "o_over_q":
+        oa = qa
+        want[b.start[-1]:] = decode(b.q.host, "f16")[b.start[-1]:]
+    if form == "strided_batch":
+        t = Buffer(gpu, np.repeat(np.repeat(b.table.host, 2, 0), 3, 1)[::-1, ::-1])
+        st, ln = Buffer(gpu, np.repeat(b.q_start.host, 2)), Buffer(gpu, b.kv_len.host[::-1].astype(np.int32))
+        batch = t.view(t.host[::-1, ::-1][::2, ::3]) + st.view(st.host[::2]) + ln.view(ln.host[::-1])
+    run(gpu, stream, ophip.AttentionPagedArgs(*qa, *b.cache_args(), *oa, *batch, 1, scale))
+    got = b.q.back(stream) if form == "o_over_q" else b.o.back(stream)
+    check(decode(got, "f16"), want, tol)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+def test_attention_paged_scales(gpu, stream, scale):
+    b = Batch(gpu, np.random.default_rng(10), "bf16", 4, 2, 64, 16, [(1, 70), (5, 33)])
+    want, tol = b.expected(1, scale)
+    check(attend(gpu, stream, b, 1, scale=scale), want, tol)
+
+
+@pytest.mark.parametrize("lens", [[(1, 50), (1, 300)], [(40, 60), (1, 300)]], ids=["few", "many"])
+def test_attention_paged_one_key_outweighs_the_others(gpu, stream, lens):
+    """Scores up to hundreds: the running maximum has to carry the sums over."""
+    b = Batch(gpu, np.random.default_rng(11), "f16", 4, 1, 128, 16, lens)
+    b.q = Buffer(gpu, (b.q.host * np.float16(20)).astype(np.float16), "f16")
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("lens", [[(1, 50), (1, 300), (1, 9)], [(40, 60), (1, 300), (20, 20)]], ids=["few", "many"])
+@pytest.mark.parametrize("dh", [64, 40])
+def test_attention_paged_bad_descriptions_stay_inside(gpu, stream, lens, dh):
+    """Page numbers that are none of the cache's, lengths beyond the table, token numbers beyond the batch or in descending
+    order: no access outside the operands, and the sequences whose description is right get their rows."""
+    b = Batch(gpu, np.random.default_rng(12), "f16", 4, 2, dh, 16, lens, junk=0.0)
+    want, tol = b.expected(1)
+    table = b.table.host.copy()
+    table[0] = 0x7FFFFFF0
+    b.table = Buffer(gpu, table)
+    got = attend(gpu, stream, b, 1)
+    first = b.start[1]
+    check(got[first:], want[first:], tol[first:])
+    for start, length in (([0, 1, 2, 0xFFFFFFFF], [50, 0xFFFFFFFF, 9]), ([5, 3, 1, 0], [50, 300, 9]), ([0, 0xFFFFFFF0, 0, 0xFFFFFFFF], [1, 1, 1])):
+        b.q_start, b.kv_len = Buffer(gpu, np.array(start, np.uint32)), Buffer(gpu, np.array(length, np.uint32))
+        attend(gpu, stream, b, 1)
+
+
+@pytest.mark.parametrize("new", [1, 12])
+def test_attention_paged_recorded_and_replayed_with_other_lengths(gpu, stream, new):
+    """One recorded launch serves growing sequences: lengths and table change on the device between replays."""
+    rng = np.random.default_rng(13)
+    lens = [(new, 900), (new, 310), (new, 450)]
+    b = Batch(gpu, rng, "f16", 8, 2, 128, 32, lens)
+    op, args = ophip.AttentionPaged(gpu), b.args(1)
+    ws = gpu.malloc(max(16, op.scheme(args, 1 << 40)))
+    own = gpu.stream()
+    op.launch(args, ws, own)
+    own.synchronize()
+    own.begin_capture()
+    op.launch(args, ws, own)
+    graph = own.end_capture()
+    for step in range(4):
+        b.lens = [(new, l - 53 * step) for _, l in lens]
+        gpu.upload(b.kv_len.mem, np.array([l for _, l in b.lens], np.uint32))
+        graph.launch(own)
+        own.synchronize()
+        want, tol = b.expected(1)
+        check(decode(b.o.back(own), "f16"), want, tol, "replay %d" % step)
+    graph.destroy()
+    own.destroy()
+
+
+def test_attention_paged_offsets_past_32_bits(gpu, stream):
+    """Pages 2.5 GiB apart: the cache reaches past 2^32 elements' bytes."""
+    dh, nkvh, page, gap, npages = 64, 2, 16, 5 << 29, 3
+    mem = [gpu.malloc(gap * (npages - 1) + nkvh * page * dh * 2) for _ in range(2)]
+    rng = np.random.default_rng(14)
+    rows = [rng.standard_normal((npages, nkvh, page, dh)).astype(np.float16) for _ in range(2)]
+    for m, r in zip(mem, rows):
+        for i in range(npages):
+            gpu.upload(m, r[i], offset=gap * i)
+    for lens in ([(1, 48)], [(40, 48)]):
+        b = Batch(gpu, rng, "f16", 4, nkvh, dh, page, lens, spare=0)
+        cache = TensorLayout(dt.F16, [npages, nkvh, page, dh], [gap, page * dh * 2, dh * 2, 2])
+        q, o = b.q.host.transpose(1, 0, 2), b.o.host.transpose(1, 0, 2)
+        run(gpu, stream, ophip.AttentionPagedArgs(*b.q.view(q), cache, mem[0], cache, mem[1], *b.o.view(o), *b.batch_args(), 1, 0.125))
+        want, tol = b.expected(1, cache=rows)
+        check(decode(b.o.back(stream), "f16"), want, tol)
+
+
+def test_attention_paged_refusals(gpu, stream):
+    rng = np.random.default_rng(15)
+    b = Batch(gpu, rng, "f16", 4, 2, 64, 16, [(1, 20), (2, 30)])
+    op = ophip.AttentionPaged(gpu)
+
+    def refused(kind, at_scheme=True, **change):
+        a = b.args(1)
+        for k, v in change.items():
+            setattr(a, k, v)
+        if at_scheme:
+            with pytest.raises(ophip.SchemeError) as e:
+                op.scheme(a, 1 << 40)
+            assert e.value.kind == kind, e.value
+        with pytest.raises(ophip.LaunchError) as e:
+            op.launch(a, None, stream)
+        assert e.value.kind == kind, e.value
+
+    good = b.args(1)
+    L = lambda lay, **c: TensorLayout(c.get("dtype", lay.dt), c.get("shape", lay.shape), c.get("strides", lay.strides))
+    refused("RankNotSupport", q_layout=TensorLayout(dt.F16, [4, 64], [128, 2]))
+    refused("RankNotSupport", k_cache_layout=TensorLayout(dt.F16, [2, 16, 64], [2048, 128, 2]))
+    refused("TypeMismatch", v_cache_layout=L(good.v_cache_layout, dtype=dt.BF16))
+    refused("TypeNotSupport", page_table_layout=L(good.page_table_layout, dtype=dt.U64))
+    refused("TypeNotSupport", kv_len_layout=L(good.kv_len_layout, dtype=dt.F32))
+    f64 = {n: L(getattr(good, n), dtype=dt.F64) for n in ("q_layout", "o_layout", "k_cache_layout", "v_cache_layout")}
+    refused("TypeNotSupport", **f64)
+    refused("ShapeMismatch", o_layout=L(good.o_layout, shape=[4, 3, 32]))
+    refused("ShapeMismatch", q_start_layout=L(good.q_start_layout, shape=[2]))
+    refused("ShapeMismatch", q_start_layout=L(good.q_start_layout, shape=[0]))
+    refused("ShapeMismatch", q_layout=L(good.q_layout, shape=[3, 3, 64]), o_layout=L(good.o_layout, shape=[3, 3, 64]))  # 3 heads over 2
+    big = {n: L(getattr(good, n), shape=list(getattr(good, n).shape[:-1]) + [1024]) for n in ("q_layout", "o_layout", "k_cache_layout", "v_cache_layout")}
+    refused("ShapeNotSupport", **big)
+    refused("ArgsNotSupport", mask=2)
+    refused("ArgsNotSupport", at_scheme=False, scale=float("nan"))
+    refused("DynamicNotSupport", at_scheme=False, scale=float("inf"))
+    refused("StridesNotSupport", at_scheme=False, q_layout=L(good.q_layout, strides=[127, 512, 2]))
+    refused("StridesNotSupport", at_scheme=False, kv_len_layout=L(good.kv_len_layout, strides=[6]))
+    refused("ShapeNotSupport", at_scheme=False, k_cache_layout=L(good.k_cache_layout, shape=[6, 2, 0, 64]), v_cache_layout=L(good.v_cache_layout, shape=[6, 2, 0, 64]))
+    for n in ("q_base", "o_base", "k_cache_base", "v_cache_base", "page_table_base", "q_start_base", "kv_len_base"):
+        refused("ArgsNotSupport", at_scheme=False, **{n: None})
+    refused("ArgsNotSupport", at_scheme=False, o_base=good.q_base + 64)        # o part over q
+    refused("ArgsNotSupport", at_scheme=False, o_base=good.k_cache_base)
+    dyn = L(good.q_layout, strides=[None, None, None])
+    dyn_args = b.args(1)
+    dyn_args.q_layout = dyn
+    assert op.scheme(dyn_args, 1 << 40) >= 0
+    refused("DynamicNotSupport", at_scheme=False, q_layout=dyn)
+    # nothing to do is fine, whatever the bases
+    none = b.args(1)
+    none.q_layout, none.o_layout = L(good.q_layout, shape=[4, 0, 64]), L(good.o_layout, shape=[4, 0, 64])
+    none.q_base = none.o_base = none.k_cache_base = None
+    op.launch(none, None, stream)
+    # a cache without pages has no keys: every row of a sequence is zero
+    bare = b.args(1)
+    bare.k_cache_layout, bare.v_cache_layout = (L(good.k_cache_layout, shape=[0, 2, 16, 64]) for _ in range(2))
+    run(gpu, stream, bare, op)
+    assert (decode(b.o.back(stream), "f16") == 0).all()
+
+
+# ---- kv_append_paged
+
+def rotated(x, pos, theta):
+    """(rope(x), |a| + |b| of each element's pair) in 64 bits; x [t, heads, dh]."""
+    if not theta:
+        return x, np.zeros_like(x)
+    half = x.shape[-1] // 2
+    ang = pos.astype(np.float64)[:, None, None] * float(np.float32(theta)) ** (-np.arange(half) / half)
+    a, b = x[..., 0::2], x[..., 1::2]
+    out, size = np.empty_like(x), np.empty_like(x)
+    out[..., 0::2], out[..., 1::2] = a * np.cos(ang) - b * np.sin(ang), a * np.sin(ang) + b * np.cos(ang)
+    size[..., 0::2] = size[..., 1::2] = np.abs(a) + np.abs(b)
+    return out, size
+
+
+def append_case(gpu, rng, kind, nkvh, dh, page, lens, pad, pos_type=np.uint32, far=100000, **form):
+    b = Batch(gpu, rng, kind, nkvh, nkvh, dh, page, lens, pad=pad, junk=0.25, **form)
+    b.k, b.v = (Buffer(gpu, encode(rng.standard_normal((b.nt, nkvh, dh)), kind), kind) for _ in range(2))
+    b.pos = Buffer(gpu, rng.integers(0, far, b.nt).astype(pos_type))
+    return b
+
+
+def append_args(b, theta):
+    return ophip.KvAppendPagedArgs(*b.k.view(b.k.host.transpose(1, 0, 2)), *b.v.view(b.v.host.transpose(1, 0, 2)), *b.pos.view(), *b.cache_args(), *b.batch_args(), theta)
+
+
+def check_append(gpu, stream, b, theta, args=None):
+    """Runs it and checks the caches: the written rows, and every other bit as it was."""
+    run(gpu, stream, args or append_args(b, theta), ophip.KvAppendPaged(gpu))
+    new_k, size = rotated(decode(b.k.host, b.kind), b.pos.host, theta)
+    got = [c.back(stream) for c in b.cache]
+    left = [c.host.copy() for c in b.cache]
+    views = lambda arrays: [np.lib.stride_tricks.as_strided(a, v.shape, v.strides) for a, v in zip(arrays, b.cache_views)]
+    gv, lv = views(got), views(left)
+    for s, (n, l) in enumerate(b.lens):
+        for i in range(max(0, n - l), n):
+            t, j = b.start[s] + i, l - n + i
+            place = (b.table.host[s, j // b.page], slice(None), j % b.page)
+            if theta:
+                w = new_k[t]
+                check(decode(gv[0][place], b.kind), w, HALF[b.kind] * np.abs(w) + 2.0 ** -20 * size[t] + 2.0 ** -25, "k of token %d" % t)
+            else:
+                assert np.array_equal(gv[0][place].view(np.uint8), b.k.host[t].view(np.uint8))
+            assert np.array_equal(gv[1][place].view(np.uint8), b.v.host[t].view(np.uint8))
+            for g, o in zip(gv, lv):
+                o[place] = g[place]
+    for g, o in zip(got, left):
+        assert np.array_equal(g.view(np.uint8), o.view(np.uint8))
+    return gv
+
+
+APPENDS = [(1, 64, 16, [(1, 1)]), (2, 128, 7, [(1, 5), (1, 0), (3, 30)]), (8, 128, 16, [(1, 400), (1, 17)]), (4, 64, 32, [(40, 40), (0, 9), (7, 3)]),
+           (3, 24, 5, [(6, 11)]), (2, 512, 4, [(3, 9)]), (2, 6, 4, [(3, 9)]), (32, 128, 64, [(9, 70)])]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("theta", [10000.0, 0.0])
+@pytest.mark.parametrize("shape", APPENDS, ids=str)
+def test_kv_append_paged(gpu, stream, shape, theta, kind):
+    check_append(gpu, stream, append_case(gpu, np.random.default_rng(20), kind, *shape, pad=2), theta)
+
+
+@pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap"])
+def test_kv_append_paged_views(gpu, stream, form):
+    b = append_case(gpu, np.random.default_rng(21), "bf16", 2, 64, 16, [(3, 20), (1, 40)], 1, token_major=form == "token_major",
+                    head_gap={"head_gap": 8, "odd_gap": 3}.get(form, 0))
+    check_append(gpu, stream, b, 500000.0)
+
+
+@pytest.mark.parametrize("pos_type,far", [(np.uint32, 1 << 32), (np.int32, 1 << 31), (np.uint64, 1 << 40), (np.int64, 1 << 20)])
+def test_kv_append_paged_far_positions(gpu, stream, pos_type, far):
+    """Angles of 10^9 radians and more: taken in f64 on both sides (up to 2^40 positions the f64 angle itself is good to 2^-15
+    turns, so positions there are whole multiples of a power of two whose low bits carry nothing)."""
+    b = append_case(gpu, np.random.default_rng(22), "f32", 2, 64, 16, [(30, 40)], 0, pos_type=pos_type, far=min(far, 1 << 20))
+    check_append(gpu, stream, b, 10000.0)
+    if far > 1 << 20:  # positions that turn the first pair by whole f64 steps only: the result is a rotation still
+        pos = (b.pos.host.astype(np.uint64) * np.uint64(far >> 20)).astype(pos_type)
+        b.pos = Buffer(gpu, pos)
+        run(gpu, stream, append_args(b, 10000.0), ophip.KvAppendPaged(gpu))
+        got = np.array([decode(b.cache[0].back(stream)[b.table.host[0, j // 16], :, j % 16], "f32") for j in range(10, 40)])
+        k = decode(b.k.host, "f32")
+        norm = lambda x: x[..., 0::2] ** 2 + x[..., 1::2] ** 2
+        assert np.allclose(norm(got), norm(k), rtol=2.0 ** -18, atol=0)
+
+
+def test_kv_append_paged_bad_descriptions_stay_inside(gpu, stream):
+    b = append_case(gpu, np.random.default_rng(23), "f16", 2, 64, 16, [(2, 50), (1, 300), (3, 9)], 1)
+    table = b.table.host.copy()
+    table[0] = 0x7FFFFFF0
+    b.table = Buffer(gpu, table)
+    run(gpu, stream, append_args(b, 10000.0), ophip.KvAppendPaged(gpu))
+    now = [c.back(stream) for c in b.cache]
+    assert (now[1] != b.cache[1].host).any(axis=(1, 3)).sum() == 4  # the four tokens of the other two sequences
+    for start, length in (([0, 1, 2, 0xFFFFFFFF], [50, 0xFFFFFFFF, 9]), ([5, 3, 1, 0], [50, 300, 9]), ([0, 0xFFFFFFF0, 0, 0xFFFFFFFF], [1, 1, 1])):
+        b.q_start, b.kv_len = Buffer(gpu, np.array(start, np.uint32)), Buffer(gpu, np.array(length, np.uint32))
+        run(gpu, stream, append_args(b, 10000.0), ophip.KvAppendPaged(gpu))
+
+
+def test_kv_append_paged_refusals(gpu, stream):
+    b = append_case(gpu, np.random.default_rng(24), "f16", 2, 64, 16, [(2, 20)], 0)
+    op = ophip.KvAppendPaged(gpu)
+
+    def refused(kind, theta=10000.0, **change):
+        a = append_args(b, theta)
+        for k, v in change.items():
+            setattr(a, k, v)
+        with pytest.raises(ophip.LaunchError) as e:
+            op.launch(a, None, stream)
+        assert e.value.kind == kind, e.value
+
+    good = append_args(b, 10000.0)
+    refused("ArgsNotSupport", theta=-1.0)
+    refused("ArgsNotSupport", theta=float("nan"))
+    refused("DynamicNotSupport", theta=float("inf"))
+    refused("ArgsNotSupport", p_base=None)
+    refused("TypeNotSupport", p_layout=TensorLayout(dt.F32, [2], [4]))
+    refused("ShapeMismatch", p_layout=TensorLayout(dt.U32, [3], [4]))
+    refused("ShapeMismatch", k_layout=TensorLayout(dt.F16, [1, 2, 64], [128, 256, 2]))
+    refused("TypeMismatch", k_layout=TensorLayout(dt.BF16, [2, 2, 64], [128, 256, 2]))
+    refused("StridesNotSupport", k_layout=TensorLayout(dt.F16, [2, 2, 64], [129, 256, 2]))
+    refused("ArgsNotSupport", k_base=good.k_cache_base)
+    for n in ("k_base", "v_base", "k_cache_base", "v_cache_base", "page_table_base", "q_start_base", "kv_len_base"):
+        refused("ArgsNotSupport", **{n: None})
+    odd = append_case(gpu, np.random.default_rng(25), "f16", 1, 5, 4, [(2, 6)], 0)
+    with pytest.raises(ophip.LaunchError) as e:
+        op.launch(append_args(odd, 10000.0), None, stream)
+    assert e.value.kind == "ShapeNotSupport"
+    check_append(gpu, stream, odd, 0.0)  # without rotation any dimension
+    still = append_args(b, 0.0)
+    still.p_base = None  # ... and no positions
+    check_append(gpu, stream, b, 0.0, still)
+
+
+# ---- qk_norm_rope
+
+def normed(x, w, pos, theta, eps):
+    """(y, tolerance without the rounding) in 64 bits"""
+    z = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
+    y, size = rotated(z, pos, theta)
+    size = size if theta else np.abs(z)
+    return y, size * ((x.shape[-1] / 2 + 8) * E + 2.0 ** -20) + 2.0 ** -25
+
+
+NORMS = [(1, 4, 1, 64), (3, 32, 8, 128), (5, 7, 0, 128), (2, 0, 3, 64), (9, 3, 2, 96), (4, 2, 2, 256), (3, 2, 1, 512), (2, 3, 1, 2), (3, 2, 2, 20), (70, 5, 1, 8)]
+
+
+@pytest.mark.parametrize("kind,weight", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("bf16", "f32"), ("f32", "f32")])
+@pytest.mark.parametrize("theta", [10000.0, 0.0])
+@pytest.mark.parametrize("shape", NORMS, ids=str)
+def test_qk_norm_rope(gpu, stream, shape, theta, kind, weight):
+    rng = np.random.default_rng(30)
+    nt, nh, nkh, dh = shape
+    check_norm(gpu, stream, rng, nt, nh, nkh, dh, kind, weight, theta)
+
+
+def check_norm(gpu, stream, rng, nt, nh, nkh, dh, kind, weight, theta, form="apart", scale=1.5, eps=1e-6):
+    fused = np.concatenate([rng.standard_normal((nt, nh * dh)) * scale, rng.standard_normal((nt, nkh * dh)) * scale, rng.standard_normal((nt, 3 if form == "odd" else 8))], 1)
+    x = Buffer(gpu, encode(fused, kind), kind)
+    parts = [x.host[:, :nh * dh].reshape(nt, nh, dh), x.host[:, nh * dh:(nh + nkh) * dh].reshape(nt, nkh, dh)]
+    parts = [np.lib.stride_tricks.as_strided(x.host[:, a:], (nt, h, dh), (x.host.strides[0], dh * x.host.itemsize, x.host.itemsize)) for a, h in ((0, nh), (nh * dh, nkh))]
+    w = [Buffer(gpu, encode(1 + 0.2 * rng.standard_normal(dh), weight), weight) for _ in range(2)]
+    pos = Buffer(gpu, rng.integers(0, 100000, nt).astype(np.uint32))
+    if form == "in_place":
+        ys, args_y = [x, x], [x.view(p) for p in parts]
+    else:
+        ys = [Buffer(gpu, np.zeros((nt, max(h, 1), dh), store(kind)), kind) for h in (nh, nkh)]
+        args_y = [y.view(y.host[:, :h]) for y, h in zip(ys, (nh, nkh))]
+    run(gpu, stream, ophip.QkNormRopeArgs(*args_y[0], *x.view(parts[0]), *w[0].view(), *args_y[1], *x.view(parts[1]), *w[1].view(), *pos.view(), eps, theta), ophip.QkNormRope(gpu))
+    for i, h in enumerate((nh, nkh)):
+        got = ys[i].back(stream)
+        if form == "in_place":
+            got = got[:, (0, nh * dh)[i]:][:, :h * dh].reshape(nt, h, dh)
+        else:
+            got = got[:, :h]
+        y, tol = normed(decode(parts[i], kind), decode(w[i].host, weight), pos.host, theta, float(np.float32(eps)))
+        check(decode(got, kind), y, tol + HALF[kind] * np.abs(y), "qk"[i])
+    if form == "in_place":
+        assert np.array_equal(x.back(stream)[:, (nh + nkh) * dh:], x.host[:, (nh + nkh) * dh:])
+
+
+@pytest.mark.parametrize("form", ["in_place", "odd"])
+@pytest.mark.parametrize("dh", [64, 128, 40])
+def test_qk_norm_rope_views(gpu, stream, form, dh):
+    """q and k views of one fused projection, in place and not, its rows on 16-byte boundaries and not."""
+    check_norm(gpu, stream, np.random.default_rng(31), 6, 4, 2, dh, "f16", "f32", 10000.0, form)
+
+
+@pytest.mark.parametrize("scale", [0.0, 1e-4, 200.0])
+def test_qk_norm_rope_small_and_large_rows(gpu, stream, scale):
+    check_norm(gpu, stream, np.random.default_rng(32), 4, 3, 2, 128, "f16", "f16", 10000.0, scale=scale, eps=1e-5)
+
+
+def test_qk_norm_rope_many_tokens(gpu, stream):
+    check_norm(gpu, stream, np.random.default_rng(33), 1500, 4, 1, 64, "bf16", "f32", 10000.0)
+
+
+def test_qk_norm_rope_refusals(gpu, stream):
+    op = ophip.QkNormRope(gpu)
+    mem = gpu.malloc(1 << 16)
+    lay = lambda h, d=64, t=dt.F16, n=2: TensorLayout.new_contiguous(t, [n, h, d])
+    w = lambda d=64, t=dt.F16: TensorLayout.new_contiguous(t, [d])
+    p = TensorLayout.new_contiguous(dt.U32, [2])
+    base = lambda i: mem.ptr + 4096 * i
+
+    def make(**change):
+        a = ophip.QkNormRopeArgs(lay(4), base(0), lay(4), base(1), w(), base(2), lay(2), base(3), lay(2), base(4), w(), base(5), p, base(6), 1e-5, 10000.0)
+        for k, v in change.items():
+            setattr(a, k, v)
+        return a
+
+    op.launch(make(), None, stream)
+    stream.synchronize()
+
+    def refused(kind, **change):
+        with pytest.raises(ophip.LaunchError) as e:
+            op.launch(make(**change), None, stream)
+        assert e.value.kind == kind, e.value
+
+    refused("ShapeMismatch", q_layout=lay(3))
+    refused("ShapeMismatch", kw_layout=w(32))
+    refused("ShapeMismatch", p_layout=TensorLayout.new_contiguous(dt.U32, [3]))
+    refused("TypeMismatch", k_layout=lay(2, t=dt.BF16))
+    refused("TypeMismatch", kw_layout=w(t=dt.F32))
+    refused("TypeNotSupport", qw_layout=w(t=dt.BF16), kw_layout=w(t=dt.BF16))
+    refused("TypeNotSupport", p_layout=TensorLayout.new_contiguous(dt.F32, [2]))
+    refused("RankNotSupport", q_layout=w())
+    odd = {n: lay(h, 63) for n, h in (("qy_layout", 4), ("q_layout", 4), ("ky_layout", 2), ("k_layout", 2))}
+    refused("ShapeNotSupport", qw_layout=w(63), kw_layout=w(63), **odd)
+    refused("StridesNotSupport", q_layout=TensorLayout(dt.F16, [2, 4, 64], [1024, 256, 4]))
+    refused("ArgsNotSupport", qy_base=base(1) + 2)
+    refused("ArgsNotSupport", theta=-3.0)
+    refused("DynamicNotSupport", epsilon=float("inf"))
+    for n in ("qy_base", "q_base", "qw_base", "ky_base", "k_base", "kw_base", "p_base"):
+        refused("ArgsNotSupport", **{n: None})
+    op.launch(make(p_base=None, theta=0.0), None, stream)
+    stream.synchronize()
+
+
+# ---- together: prompts of two sequences, then decode steps, each step norm + rope, append, attention over the cache
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_prompt_and_decode_steps_over_a_paged_cache(gpu, stream, kind):
+    rng = np.random.default_rng(40)
+    nh, nkvh, dh, page, theta, eps = 8, 2, 64, 16, 10000.0, 1e-6
+    npages, cols = 12, 5
+    u = HALF[kind]
+    table = Buffer(gpu, rng.permutation(npages)[:2 * cols].reshape(2, cols).astype(np.uint32))
+    cache = [Buffer(gpu, encode(np.full((npages, nkvh, page, dh), np.nan), kind), kind) for _ in range(2)]
+    w = [Buffer(gpu, encode(1 + 0.2 * rng.standard_normal(dh), "f32"), "f32") for _ in range(2)]
+    norm, append, attention = ophip.QkNormRope(gpu), ophip.KvAppendPaged(gpu), ophip.AttentionPaged(gpu)
+    past = [[[], []], [[], []]]  # per sequence: its keys and values as the cache holds them, in 64 bits
+    length = [0, 0]
+    for new in ([37, 20], [1, 1], [1, 1], [1, 0], [5, 30]):
+        nt = sum(new)
+        length = [l + n for l, n in zip(length, new)]
+        start = np.concatenate([[0], np.cumsum(new)]).astype(np.uint32)
+        pos = np.concatenate([np.arange(l - n, l) for l, n in zip(length, new)]).astype(np.uint32)
+        qkv = Buffer(gpu, encode(rng.standard_normal((nt, (nh + 2 * nkvh) * dh)), kind), kind)
+        heads = lambda a, h: np.lib.stride_tricks.as_strided(a[:, 0:], (nt, h, dh), (qkv.host.strides[0], dh * SIZE[kind], SIZE[kind]))
+        q, k, v = heads(qkv.host, nh), heads(qkv.host[:, nh * dh:], nkvh), heads(qkv.host[:, (nh + nkvh) * dh:], nkvh)
+        o = Buffer(gpu, np.zeros((nt, nh, dh), store(kind)), kind)
+        st, ln, ps = Buffer(gpu, start), Buffer(gpu, np.array(length, np.uint32)), Buffer(gpu, pos)
+        batch, caches = table.view() + st.view() + ln.view(), cache[0].view() + cache[1].view()
+        norm.launch(ophip.QkNormRopeArgs(*qkv.view(q), *qkv.view(q), *w[0].view(), *qkv.view(k), *qkv.view(k), *w[1].view(), *ps.view(), eps, theta), None, stream)
+        append.launch(ophip.KvAppendPagedArgs(*qkv.view(k.transpose(1, 0, 2)), *qkv.view(v.transpose(1, 0, 2)), *ps.view(), *caches, *batch, 0.0), None, stream)
+        attention.launch(ophip.AttentionPagedArgs(*qkv.view(q.transpose(1, 0, 2)), *caches, *o.view(o.host.transpose(1, 0, 2)), *batch, 1, dh ** -0.5), None, stream)
+        stream.synchronize()
+        got_o, got_qkv = decode(o.back(stream), kind), qkv.back(stream)
+        # each step's inputs to the next are checked, and taken as they came out
+        for i, (a, h) in enumerate(((0, nh), (nh * dh, nkvh))):
+            y, tol = normed(decode(heads(qkv.host[:, a:], h), kind), decode(w[i].host, "f32"), pos, theta, eps)
+            check(decode(heads(got_qkv[:, a:], h), kind), y, tol + u * np.abs(y))
+        qn, kn, vn = decode(heads(got_qkv, nh), kind), decode(heads(got_qkv[:, nh * dh:], nkvh), kind), decode(v, kind)
+        for s in range(2):
+            for t in range(start[s], start[s + 1]):
+                past[s][0].append(kn[t])
+                past[s][1].append(vn[t])
+                keys, values = np.array(past[s][0]), np.array(past[s][1])
+                for h in range(nh):
+                    kk, vv = keys[:, h // 4], values[:, h // 4]
+                    x = kk @ qn[t, h] * dh ** -0.5
+                    pr = np.exp(x - x.max())
+                    pr /= pr.sum()
+                    big = (np.abs(kk) @ np.abs(qn[t, h])).max() * dh ** -0.5
+                    check(got_o[t, h], pr @ vv, (2 * u + 2 * (dh + 8) * E * big + 2.0 ** -20) * (pr @ np.abs(vv)) + 2.0 ** -25, "token %d head %d" % (t, h))
+
+
+def test_two_streams_share_the_operators(gpu):
+    """One operator on two streams with a workspace each: neither sees the other's partial results."""
+    rng = np.random.default_rng(41)
+    op = ophip.AttentionPaged(gpu)
+    jobs = []
+    for lens in ([(1, 2000)], [(1, 1500), (1, 900)]):
+        b = Batch(gpu, rng, "f16", 4, 1, 64, 16, lens)
+        args, s = b.args(1), gpu.stream()
+        jobs.append((b, args, s, gpu.malloc(max(16, op.scheme(args, 1 << 40)))))
+    for _ in range(3):
+        for b, args, s, ws in jobs:
+            op.launch(args, ws, s)
+    for b, args, s, ws in jobs:
+        want, tol = b.expected(1)
+        check(decode(b.o.back(s), "f16"), want, tol)
+        s.destroy()
+
+
+def test_a_stream_made_elsewhere(gpu):
+    """ExternalStream takes a hipStream_t it did not make: the operators run on it."""
+    own = gpu.stream()
+    s = ophip.ExternalStream(gpu, own.handle.value)
+    b = Batch(gpu, np.random.default_rng(42), "f16", 2, 1, 64, 16, [(1, 40)])
+    ophip.AttentionPaged(gpu).launch(b.args(1), None, s)
+    own.synchronize()
+    want, tol = b.expected(1)
+    check(decode(b.o.back(own), "f16"), want, tol)
+    own.destroy()
+
+
+def test_null_operators_and_arguments(gpu):
+    L = ophip.lib()
+    ws = ctypes.c_size_t(0)
+    for n in ("attention_paged", "kv_append_paged", "qk_norm_rope"):
+        assert getattr(L, "ophip_%s_create" % n)(None, None) == 8
+        assert getattr(L, "ophip_%s_launch" % n)(None, None, None, ctypes.c_size_t(0), None) == 8
+        assert getattr(L, "ophip_%s_scheme" % n)(None, None, ctypes.c_size_t(0), ctypes.byref(ws)) == 8
+        getattr(L, "ophip_%s_destroy" % n)(None)
