@@ -3,6 +3,8 @@
 // operators take one sequence at a time; names, layouts, verbs and errors follow the crate's operators.
 #include <algorithm>
 #include <cmath>
+#include <cstdio>
+#include <cstdlib>
 
 #include "../kernels/params.h"
 #include "handle.hpp"
@@ -121,10 +123,21 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 
 struct ophip_attention_paged : OpBase {
     hipFunction_t any[3];
+    hipFunction_t rows[2][2][2], join[2][2][2];  // [f16 / bf16][tiles of 16 / 128 rows][dh 64 / 128]
+    int slots[2] = {0, 0};  // OPHIP_ATTN_PAGED_SLOTS=<few>,<many>: key ranges to cut a launch into (sweeps); read once, here
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
         any[0] = d->kernel("attention_paged_any", "attn_paged_any_f16");
         any[1] = d->kernel("attention_paged_any", "attn_paged_any_bf16");
         any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
+        for (int e = 0; e < 2; ++e)
+            for (int r = 0; r < 2; ++r)
+                for (int h = 0; h < 2; ++h) {
+                    const char *mod = e ? "attention_paged_bf16" : "attention_paged";
+                    const std::string tail = std::string(r ? "many" : "few") + (h ? "_d128" : "_d64") + (e ? "_bf16" : "");
+                    rows[e][r][h] = d->kernel(mod, ("attn_paged_" + tail).c_str());
+                    join[e][r][h] = d->kernel(mod, ("attn_paged_join_" + tail).c_str());
+                }
+        if (const char *e = std::getenv("OPHIP_ATTN_PAGED_SLOTS")) std::sscanf(e, "%d,%d", &slots[0], &slots[1]);
     }
 };
 
@@ -148,6 +161,39 @@ AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
     if (!is_dyn(m.nh) && !is_dyn(m.nkvh) && (m.nkvh == 0 ? m.nh != 0 : m.nh % m.nkvh != 0)) throw shape_mismatch("nh must be a multiple of nkvh");
     if (!is_dyn(m.dh) && m.dh > MAX_HEAD) throw shape_not_support("head dimension too large");
     return m;
+}
+
+// How the matrix kernels take a call (attention_paged.hip), from its sizes alone.
+struct AttnPagedPlan {
+    bool matrix;                    // they serve these types and sizes
+    int many;                       // tiles of 128 rows, or of 16
+    size_t grid, slots, min_steps;  // workgroups; key ranges the workspace holds (0: no tile can be cut); steps of 32 keys a range has at least
+    size_t workspace;
+};
+AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPagedMeta &m) {
+    AttnPagedPlan a{};
+    for (size_t v : {m.nh, m.nt, m.dh, m.nkvh, m.nseq, m.page, m.cols})
+        if (is_dyn(v) || v == 0) return a;
+    if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || (m.dh != 64 && m.dh != 128) || m.nh % m.nkvh) return a;
+    if (m.nh > MAX_INDEX / m.nt || m.page > MAX_INDEX / m.cols) return a;
+    a.matrix = true;
+    // up to 16 rows per sequence and kv head on average: nearly all of it is decode steps
+    const size_t group = m.nh / m.nkvh, rows = m.nt * group;
+    a.many = rows > 16 * m.nseq;
+    const size_t tile = a.many ? 128 : 16;
+    // the most tiles there can be, whatever the lengths: each sequence that has a token may have one that is not full
+    const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
+    const size_t steps = (m.cols * m.page + 31) / 32;
+    a.min_steps = a.many ? 8 : 4;
+    const size_t most = std::max<size_t>(1, steps / a.min_steps);
+    const size_t want = op && op->slots[a.many] > 0 ? (size_t)op->slots[a.many] : 2 * (size_t)(op ? op->dev->props.multiProcessorCount : 256);
+    a.grid = units;
+    if (most > 1) {
+        a.slots = std::min(2 * want, units * most);
+        a.grid = std::min(units * most, units + 2 * want);
+        a.workspace = 64 + a.slots * (32 + tile * (m.dh + 2) * sizeof(float));
+    }
+    return a;
 }
 
 void attention_paged_launch(const ophip_attention_paged *op, const ophip_attention_paged_args &a, void *workspace, size_t workspace_len,
@@ -183,6 +229,19 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     p.group = make_fastdiv((uint32_t)(nh / nkvh));
     p.nkvh = (uint32_t)nkvh, p.dh = (uint32_t)dh, p.causal = a.mask == OPHIP_MASK_CAUSAL;
     p.scale = scale;
+    const AttnPagedPlan plan = attention_paged_plan(op, m);
+    // (a scale that is not positive: the matrix kernels take the maximum before they scale)
+    if (plan.matrix && p.b.cols && scale > 0.f && plan.grid <= MAX_INDEX && vector_rows(a.q_layout, a.q_base) && vector_rows(a.o_layout, a.o_base) &&
+        vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base)) {
+        Workspace ws(qa, workspace, workspace_len, plan.workspace);
+        p.work = ws.ptr();
+        p.slots = (uint32_t)plan.slots, p.min_steps = (uint32_t)plan.min_steps;
+        const int e = m.dt == OPHIP_DT_BF16, h = dh == 128;
+        op->dev->make_current();
+        launch(op->rows[e][plan.many][h], Dim3{(unsigned)plan.grid}, Dim3{256}, 0, stream_of(qa), p);
+        if (plan.slots) launch(op->join[e][plan.many][h], Dim3{(unsigned)plan.slots, plan.many ? 4u : 1u}, Dim3{256}, 0, stream_of(qa), p);
+        return;
+    }
     op->dev->make_current();
     launch(op->any[type_index(m.dt)], Dim3{(unsigned)(nt * nh)}, Dim3{256}, 0, stream_of(qa), p);
 }
@@ -203,7 +262,9 @@ int ophip_attention_paged_scheme(ophip_attention_paged *op, const ophip_attentio
     return guard([&] {
         if (ws) *ws = 0;
         if (!args) throw args_not_support("null argument");
-        (void)attention_paged_meta(*args);
+        const AttnPagedMeta m = attention_paged_meta(*args);
+        const size_t need = attention_paged_plan(op, m).workspace;
+        if (ws && need <= max_ws) *ws = need;  // (with less, launch takes it from the queue's allocator)
     });
 }
 

@@ -1,0 +1,537 @@
+// attention over a paged cache on the matrix cores: o = softmax(scale q . k^T) . v for a packed batch of sequences of
+// unlike lengths, f16 / bf16, dh 64 and 128.
+//
+// Work units.  The query rows of one kv head and sequence are its new tokens times the `group` query heads that share
+// the kv head, row = token * group + head-in-group, cut into tiles of 16 rows (attn_paged_few: decode steps, where the
+// caches are all the traffic) or 128 (attn_paged_many: prompts and chunks, where the products are the work).  So keys and
+// values are read once per tile whatever the group, and a short group fills the rows with further tokens.
+//
+// Plan.  The host knows the number of tokens and sequences, not the lengths, and must not wait for them; so every
+// workgroup works its own unit out from the lengths on the device (paged_item: two prefix sums over the sequences, about a
+// microsecond): the tiles of a sequence with more keys than 1 / slots of all tiles' keys are cut into that many more
+// key ranges, one workgroup each, so that a launch has about `slots` equal pieces of work whatever the mix of lengths.
+// Ranges of a cut tile leave their maximum, sum and output in the workspace and attn_paged_join merges them in a fixed
+// order: results do not depend on which workgroup ends first.
+//
+// Compiled twice, like the other MFMA kernels (gemm_elem.h).
+#include "gemm_elem.h"
+#include "paged.h"
+
+constexpr float PA_LOG2E = 1.4426950408889634f;
+// Probabilities are kept times 2^PA_BIAS (as are their sums): in f16, 2^-25 steps below 2^-14 would cost the many small
+// ones of a long row their bits.
+#ifdef GEMM_ELEM_BF16
+constexpr float PA_BIAS = 0.f;
+#else
+constexpr float PA_BIAS = 15.f;
+#endif
+
+// ---- the workspace: a count, a descriptor per slot (32 bytes), then per slot ROWS pairs (maximum, sum), then per slot
+// ROWS rows of DH floats
+struct PagedDesc {
+    uint32_t piece, pieces, kvh, row0, nrows, start, _pad[2];
+};
+__device__ __forceinline__ PagedDesc *paged_desc(const AttnPagedParams &p) { return reinterpret_cast<PagedDesc *>(reinterpret_cast<char *>(p.work) + 64); }
+__device__ __forceinline__ float *paged_stats(const AttnPagedParams &p) { return reinterpret_cast<float *>(reinterpret_cast<char *>(p.work) + 64 + 32 * (size_t)p.slots); }
+__device__ __forceinline__ float *paged_partial(const AttnPagedParams &p, int rows) { return paged_stats(p) + 2 * (size_t)rows * p.slots; }
+
+struct PagedItem {
+    PagedSeq s;
+    uint32_t seq, kvh, piece, pieces, slot;  // slot: where the range's result goes, when pieces > 1
+    uint32_t row0, nrows;                     // rows of the sequence and kv head
+};
+
+// What workgroup blockIdx.x does; false: nothing.  Every thread of the 256 or more calls it and gets the same.
+template <int ROWS>
+__device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &it) {
+    __shared__ uint64_t s_work[4];
+    __shared__ uint32_t s_scan[2][4], s_found[4];
+    const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE, w = blockIdx.x;
+    auto tiles_of = [&](const PagedSeq &s) { return (uint32_t)(((uint64_t)s.n * p.group.d + ROWS - 1) / ROWS); };
+    auto steps_of = [&](const PagedSeq &s) { return (s.len + 31) / 32; };
+    float per_step = 0.f;  // key ranges per step of 32 keys
+    if (tid == 0) s_found[0] = 0xffffffffu;
+    if (p.slots) {
+        uint64_t work = 0;
+        for (uint32_t i = tid; i < p.b.nseq; i += 256) {
+            const PagedSeq s = paged_seq(p.b, i);
+            work += (uint64_t)tiles_of(s) * steps_of(s);
+        }
+        work = wave_sum(work);
+        if (lane == 0) s_work[wave] = work;
+        __syncthreads();
+        work = s_work[0] + s_work[1] + s_work[2] + s_work[3];
+        // half the slots: a count rounded up from more than one is less than twice as much
+        if (work) per_step = 0.4999995f * (float)p.slots / ((float)work * (float)p.nkvh);
+    } else __syncthreads();
+    uint32_t items0 = 0, slots0 = 0;
+    for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += 256) {
+        uint32_t items = 0, slots = 0, pieces = 1;
+        if (i0 + tid < p.b.nseq) {
+            const PagedSeq s = paged_seq(p.b, i0 + tid);
+            const uint32_t most = steps_of(s) / p.min_steps;
+            if (p.slots && most > 1) pieces = min(most, max(1u, (uint32_t)ceilf((float)steps_of(s) * per_step)));
+            items = tiles_of(s) * p.nkvh * pieces;
+            slots = pieces > 1 ? items : 0;
+        }
+        uint32_t a = items, b = slots;
+#pragma unroll
+        for (int o = 1; o < WAVE; o <<= 1) {
+            const uint32_t ua = __shfl_up(a, o, WAVE), ub = __shfl_up(b, o, WAVE);
+            if (lane >= (uint32_t)o) a += ua, b += ub;
+        }
+        if (lane == WAVE - 1) s_scan[0][wave] = a, s_scan[1][wave] = b;
+        __syncthreads();
+        uint32_t ta = 0, tb = 0;
+#pragma unroll
+        for (uint32_t v = 0; v < 4; ++v) {
+            if (v < wave) a += s_scan[0][v], b += s_scan[1][v];
+            ta += s_scan[0][v], tb += s_scan[1][v];
+        }
+        const uint32_t before = items0 + a - items;
+        if (w - before < items) s_found[0] = i0 + tid, s_found[1] = w - before, s_found[2] = pieces, s_found[3] = slots0 + b - slots;
+        items0 += ta, slots0 += tb;
+        __syncthreads();
+        if (w < items0 && w != 0) break;  // (workgroup 0 counts all slots)
+    }
+    if (w == 0 && tid == 0 && p.slots) *reinterpret_cast<uint32_t *>(p.work) = min(slots0, p.slots);
+    if (s_found[0] == 0xffffffffu) return false;
+    it.seq = __builtin_amdgcn_readfirstlane(s_found[0]);
+    const uint32_t local = __builtin_amdgcn_readfirstlane(s_found[1]);
+    it.pieces = __builtin_amdgcn_readfirstlane(s_found[2]);
+    it.slot = __builtin_amdgcn_readfirstlane(s_found[3]) + local;
+    if (it.pieces > 1 && it.slot >= p.slots) return false;
+    it.s = paged_seq(p.b, it.seq);
+    // kv heads next to each other (consecutive workgroups go to different XCDs, so a kv head's tiles meet in one L2), a
+    // tile's ranges next, the tiles last to first: the last has the most keys under a causal mask
+    it.kvh = local % p.nkvh;
+    const uint32_t rest = local / p.nkvh, rows = it.s.n * p.group.d, back = rest / it.pieces;
+    it.piece = rest - back * it.pieces;
+    it.row0 = (tiles_of(it.s) - 1 - back) * ROWS;
+    it.nrows = min((uint32_t)ROWS, rows - it.row0);
+    if (it.pieces > 1 && tid == 0) paged_desc(p)[it.slot] = PagedDesc{it.piece, it.pieces, it.kvh, it.row0, it.nrows, it.s.start, {0, 0}};
+    return true;
+}
+
+// Keys that a row (of the sequence and kv head) keeps
+__device__ __forceinline__ uint32_t paged_keep(const AttnPagedParams &p, const PagedItem &it, uint32_t token) {
+    if (!p.causal) return it.s.len;
+    const int64_t keep = (int64_t)it.s.len - it.s.n + token + 1;
+    return keep < 0 ? 0 : (uint32_t)keep;
+}
+
+// ---- up to 16 rows: one pass over the keys at the rate of memory
+//
+// A workgroup of four waves takes a key range in steps of 32 keys, a step per wave; nothing is shared between the waves
+// until the end.  Keys and values go from memory straight into the lanes' registers, the next step's on their way while one
+// is multiplied, and the page numbers one step ahead of those.
+//   S^T = K . Q^T (v_mfma 16x16x32): A is 16 keys, 16 bytes per lane as they lie in memory; lane (j, g) of the result has
+//   query j and the keys 4 g + i of the 16.  So a query's maximum and sum are eight registers of four lanes, its
+//   factors are scalars of the lane, and the probabilities are, as they lie, B operands of
+//   O^T = V^T . P^T, contraction slot 8 g + 4 c + i being key 16 c + 4 g + i.  A is then the values of those eight keys, of
+//   which the lane reads DH / 16 adjacent columns each and transposes them in registers.
+// The matrix cores are idle most of the time: 16 KB of keys and values take about 500 cycles of one wave, a CU's share of
+// the memory's rate delivers them in 1300.
+template <int CW>
+struct FewTile {  // 32 keys
+    u32x4 k[2][CW / 2];
+    uint32_t v[8][CW / 2];
+};
+
+template <int DH>
+__device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
+    constexpr int CW = DH / 16, KS = DH / 32;  // columns of v per lane, contraction steps of q . k
+    __shared__ float s_m[4][16], s_l[4][16], s_o[4][CW * 4][WAVE];
+    PagedItem it;
+    if (!paged_item<16>(p, it)) return;
+    const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, j = lane % 16, g = lane / 16;
+    const uint32_t row = it.row0 + min(j, it.nrows - 1), token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
+    const uint32_t keep = paged_keep(p, it, token), keys = paged_keep(p, it, fastdiv(it.row0 + it.nrows - 1, p.group));
+    const uint32_t steps = (keys + 31) / 32, per = (steps + it.pieces - 1) / it.pieces;
+    const uint32_t first = it.piece * per + wave, last = min(steps, it.piece * per + per);
+
+    u32x4 q[KS];
+    {
+        const char *src = reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st + 16 * g;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = ld128(src + 64 * s);
+    }
+    const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 16 * g;
+    const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 2 * CW * j;
+    // the lane's two keys of a step (16 c + j), bounded by the sequence's last
+    uint32_t col[2], line[2], page[2];
+    auto look_up = [&](uint32_t step) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const uint32_t key = min(step * 32 + 16 * c + j, it.s.len - 1);
+            col[c] = fastdiv(key, p.b.page);
+            line[c] = key - col[c] * p.b.page.d;
+            page[c] = paged_page(p.b, it.seq, col[c]);
+        }
+    };
+    auto fetch = [&](FewTile<CW> &t) {
+        uint32_t pg[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            pg[c] = min(page[c], p.b.npages - 1);
+            const char *src = kb + (int64_t)pg[c] * p.k_sp + (int64_t)line[c] * p.k_sr;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) t.k[c][s] = ld128(src + 64 * s);
+        }
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t vp = __shfl(pg[c], 4 * g + i, WAVE), vl = __shfl(line[c], 4 * g + i, WAVE);
+                const char *src = vb + (int64_t)vp * p.v_sp + (int64_t)vl * p.v_sr;
+                if constexpr (CW == 8) *reinterpret_cast<u32x4 *>(t.v[4 * c + i]) = ld128(src);
+                else *reinterpret_cast<u32x2 *>(t.v[4 * c + i]) = *reinterpret_cast<const u32x2 *>(src);
+            }
+    };
+    const float scale2 = p.scale * PA_LOG2E;
+    float m = -INFINITY, l = 0.f;
+    f32x4 o[CW];
+#pragma unroll
+    for (int t = 0; t < CW; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const FewTile<CW> &t, uint32_t step) {
+        float x[8], mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                PackE a, b;
+                a.u = t.k[c][k];
+                b.u = q[k];
+                s = mfma_16x16x32(a.h, b.h, s);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                x[4 * c + i] = step * 32 + 16 * c + 4 * g + i < keep ? s[i] * scale2 : -INFINITY;
+                mx = fmaxf(mx, x[4 * c + i]);
+            }
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+        const float top = fmaxf(m, mx), ref = top == -INFINITY ? 0.f : top;
+        if (__builtin_amdgcn_ballot_w64(top != m) != 0) {
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+            l *= f;
+#pragma unroll
+            for (int c = 0; c < CW; ++c) o[c] *= f;
+            m = top;
+        }
+        PackE pr;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float e = __builtin_amdgcn_exp2f(x[i] - ref + PA_BIAS);
+            l += e;
+            pr.e[i] = f2e(e);
+        }
+#pragma unroll
+        for (int c = 0; c < CW; ++c) {
+            PackE a;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t lo = t.v[2 * d][c / 2], hi = t.v[2 * d + 1][c / 2];
+                a.u[d] = (c & 1) ? ((lo >> 16) | (hi & 0xffff0000u)) : ((lo & 0xffffu) | (hi << 16));
+            }
+            o[c] = mfma_16x16x32(a.h, pr.h, o[c]);
+        }
+    };
+    if (first < last) {
+        FewTile<CW> a, b;
+        look_up(first);
+        fetch(a);
+        look_up(first + 4);
+        for (uint32_t step = first; step < last; step += 8) {
+            if (step + 4 < last) {
+                fetch(b);
+                look_up(step + 8);
+            }
+            multiply(a, step);
+            if (step + 4 < last) {
+                if (step + 8 < last) {
+                    fetch(a);
+                    look_up(step + 12);
+                }
+                multiply(b, step + 4);
+            }
+        }
+    }
+    l += __shfl_xor(l, 16, WAVE);
+    l += __shfl_xor(l, 32, WAVE);
+
+    // the four waves' results, on one maximum
+    if (g == 0) s_m[wave][j] = m, s_l[wave][j] = l;
+    __syncthreads();
+    float top = s_m[0][j];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][j]);
+    const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m - ref);
+    float total = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) total += s_l[w][j] * __builtin_amdgcn_exp2f(s_m[w][j] - ref);
+#pragma unroll
+    for (int t = 0; t < CW; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s_o[wave][4 * t + i][lane] = o[t][i] * f;
+    __syncthreads();
+    // lane (j, g) of wave i: query j, columns CW (4 g + i) .. + CW - 1
+    if (j >= it.nrows) return;
+    float out[CW];
+#pragma unroll
+    for (int t = 0; t < CW; ++t) {
+        out[t] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) out[t] += s_o[w][4 * t + wave][lane];
+    }
+    const uint32_t column = CW * (4 * g + wave);
+    if (it.pieces > 1) {
+        float *dst = paged_partial(p, 16) + ((size_t)it.slot * 16 + j) * DH + column;
+#pragma unroll
+        for (int t = 0; t < CW; t += 4) *reinterpret_cast<f32x4 *>(dst + t) = f32x4{out[t], out[t + 1], out[t + 2], out[t + 3]};
+        if (column == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * 16 + j) * 2) = f32x2{top, total};
+        return;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
+    union {
+        elem e[CW];
+        u32x4 u4;
+        u32x2 u2;
+    } y;
+#pragma unroll
+    for (int t = 0; t < CW; ++t) y.e[t] = f2e(out[t] * inv);
+    char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 2 * column;
+    if constexpr (CW == 8) st128(dst, y.u4);
+    else *reinterpret_cast<u32x2 *>(dst) = y.u2;
+}
+
+// ---- up to 128 rows: the products are the work
+//
+// A workgroup of four waves, 32 rows each, walks its key range in tiles of 64 keys that go through registers into LDS,
+// double-buffered, one barrier a tile; two workgroups share a CU.  S^T = K . Q^T with v_mfma 32x32x16: a lane holds one
+// query and half the tile's keys, so maxima, sums and factors are scalars of the lane; the probabilities are packed in
+// registers into B operands of O^T = V^T . P^T, whose A operands come from the row-major tile through the transposing
+// LDS read.  A wave without rows, or whose rows all end before a tile, only helps to load.
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int DH>
+__device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
+    constexpr int BN = 64;
+    constexpr int KP = DH + 8, VP = DH + 32;  // pitches of a row in LDS: reads of consecutive rows spread over the banks
+    constexpr int CPR = DH / 8, NCH = BN * CPR / 256, RS = 256 / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
+    constexpr int DS = DH / 16, DB = DH / 32;
+    __shared__ __attribute__((aligned(16))) elem k_lds[2][BN * KP];
+    __shared__ __attribute__((aligned(16))) elem v_lds[2][BN * VP];
+    PagedItem it;
+    if (!paged_item<128>(p, it)) return;
+    const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+    const uint32_t n32 = lane % 32, h = lane / 32, s16 = lane % 16, b16 = (lane / 16) % 2;
+    const uint32_t wrow = wave * 32, at = min(wrow + n32, it.nrows - 1);
+    const uint32_t row = it.row0 + at, token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
+    const uint32_t keys = paged_keep(p, it, fastdiv(it.row0 + it.nrows - 1, p.group));
+    const int32_t lim = (int32_t)paged_keep(p, it, token);  // the lane's row keeps keys below it ...
+    const int32_t lim_first = __builtin_amdgcn_readfirstlane(lim);  // ... the wave's first row, which keeps the fewest ...
+    const int32_t lim_last = wrow < it.nrows ? (int32_t)paged_keep(p, it, fastdiv(it.row0 + min(wrow + 31, it.nrows - 1), p.group)) : 0;  // ... its last
+    const uint32_t tiles = (keys + BN - 1) / BN, per = (tiles + it.pieces - 1) / it.pieces;
+    const uint32_t first = it.piece * per, last = min(tiles, first + per);
+
+    PackE qf[DS];
+    {
+        const char *src = reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st + 16 * h;
+#pragma unroll
+        for (int d = 0; d < DS; ++d) qf[d].u = ld128(src + 32 * d);
+    }
+    const uint32_t cc = tid % CPR, cr = tid / CPR;
+    const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 16 * cc;
+    const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 16 * cc;
+    uint32_t line[NCH], page[NCH];
+    u32x4 kreg[NCH], vreg[NCH];
+    auto look_up = [&](uint32_t t) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t key = min(t * BN + cr + RS * i, it.s.len - 1), col = fastdiv(key, p.b.page);
+            line[i] = key - col * p.b.page.d;
+            page[i] = paged_page(p.b, it.seq, col);
+        }
+    };
+    auto fetch = [&]() {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            const uint32_t pg = min(page[i], p.b.npages - 1);
+            kreg[i] = ld128(kb + (int64_t)pg * p.k_sp + (int64_t)line[i] * p.k_sr);
+            vreg[i] = ld128(vb + (int64_t)pg * p.v_sp + (int64_t)line[i] * p.v_sr);
+        }
+    };
+    auto commit = [&](int buf) {
+#pragma unroll
+        for (int i = 0; i < NCH; ++i) {
+            st128(&k_lds[buf][(cr + RS * i) * KP + 8 * cc], kreg[i]);
+            st128(&v_lds[buf][(cr + RS * i) * VP + 8 * cc], vreg[i]);
+        }
+    };
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float scale2 = p.scale * PA_LOG2E;  // (positive: maxima commute with it)
+
+    if (first < last) {
+        look_up(first);
+        fetch();
+        commit(0);
+        if (first + 1 < last) look_up(first + 1);
+    }
+    __syncthreads();
+    for (uint32_t t = first; t < last; ++t) {
+        const int buf = (t - first) & 1;
+        const bool more = t + 1 < last;
+        if (more) {
+            fetch();
+            look_up(t + 2);
+        }
+        if ((int32_t)(t * BN) < lim_last) {
+            const elem *kt = k_lds[buf], *vt = v_lds[buf];
+            // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
+            f32x16 sacc[2];
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sacc[b][e] = 0.f;
+#pragma unroll
+                for (int d = 0; d < DS; ++d) {
+                    PackE a;
+                    a.u = ld128(kt + (32 * b + n32) * KP + 16 * d + 8 * h);
+                    sacc[b] = mfma_32x32x16(a.h, qf[d].h, sacc[b]);
+                }
+            }
+            if ((int32_t)(t * BN + BN) > lim_first) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        if ((int32_t)(t * BN + 32 * b + 8 * (e / 4) + 4 * h + e % 4) >= lim) sacc[b][e] = -INFINITY;
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sacc[b][e]);
+            mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
+            const float top = fmaxf(m, mx * scale2), ref = top == -INFINITY ? 0.f : top;
+            if (__builtin_amdgcn_ballot_w64(top != m) != 0) {
+                const float f = __builtin_amdgcn_exp2f(m - ref);
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[d][e] *= f;
+                m = top;
+            }
+            const float shift = PA_BIAS - ref;
+            float sum = 0.f;
+            PackE pb[4];  // MFMA n: the tile's keys 16 n .. + 15, slots 8 h .. 8 h + 7 keys 16 n + 4 h + {0..3}, 16 n + 8 + 4 h + {0..3}
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift));
+                    sum += x;
+                    pb[2 * b + e / 8].e[e % 8] = f2e(x);
+                }
+            l += sum;
+            typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const elem *src = vt + (16 * n + 4 * h + s16 / 4) * VP + 32 * d + 16 * b16 + 4 * (s16 % 4);
+                    union {
+                        s16x4 half[2];
+                        elem8 hv;
+                    } a;
+                    a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)src);
+                    a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(src + 8 * VP));
+                    o[d] = mfma_32x32x16(a.hv, pb[n].h, o[d]);
+                }
+        }
+        if (more) commit(buf ^ 1);
+        __syncthreads();
+    }
+    const float total = l + __shfl_xor(l, 32, WAVE);
+    if (wrow + n32 >= it.nrows) return;
+    // o[d][4 q + r]: column 32 d + 8 q + 4 h + r of the lane's query
+    if (it.pieces > 1) {
+        float *dst = paged_partial(p, 128) + ((size_t)it.slot * 128 + at) * DH + 4 * h;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * q) = f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+        if (h == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * 128 + at) * 2) = f32x2{m, total};
+        return;
+    }
+    const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
+    char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 8 * h;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            union {
+                elem e[4];
+                u32x2 u;
+            } y;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y.e[r] = f2e(o[d][4 * q + r] * inv);
+            *reinterpret_cast<u32x2 *>(dst + 64 * d + 16 * q) = y.u;
+        }
+}
+
+// ---- the ranges of a cut tile: o = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
+//
+// Workgroup (slot, y): the rows of the slot's tile are dealt out to the workgroups of its ranges, a wave to a row, its lanes
+// the columns.
+template <int DH, int ROWS>
+__device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
+    constexpr int W = DH / WAVE;  // columns per lane
+    const uint32_t slot = blockIdx.x, wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+    const PagedDesc d = paged_desc(p)[slot];
+    // Slots behind the count hold no descriptor; nor do those of a batch whose sequences overlap, when it has more tiles than
+    // the grid allows for: what lies there must not lead outside the workspace or o.
+    if (slot >= *reinterpret_cast<const uint32_t *>(p.work) || d.pieces < 2 || d.pieces > p.slots || d.piece >= d.pieces || d.kvh >= p.nkvh || d.nrows > ROWS) return;
+    const uint64_t before = (uint64_t)d.piece * p.nkvh, behind = (uint64_t)(d.pieces - 1 - d.piece) * p.nkvh;
+    if (before > slot || slot + behind >= p.slots) return;
+    const uint32_t slot0 = slot - (uint32_t)before;
+    for (uint32_t r = (d.piece * gridDim.y + blockIdx.y) * 4 + wave; r < d.nrows; r += d.pieces * gridDim.y * 4) {
+        const float *st = paged_stats(p) + ((size_t)slot0 * ROWS + r) * 2, *po = paged_partial(p, ROWS) + ((size_t)slot0 * ROWS + r) * DH + W * lane;
+        const size_t step = (size_t)p.nkvh * ROWS;
+        float top = -INFINITY;
+        for (uint32_t c = lane; c < d.pieces; c += WAVE) top = fmaxf(top, st[2 * step * c]);
+        top = wave_max(top);
+        const float ref = top == -INFINITY ? 0.f : top;
+        float total = 0.f, out[W] = {};
+#pragma unroll 8
+        for (uint32_t c = 0; c < d.pieces; ++c) {
+            const float f = __builtin_amdgcn_exp2f(st[2 * step * c] - ref);
+            total += f * st[2 * step * c + 1];
+#pragma unroll
+            for (int i = 0; i < W; ++i) out[i] += f * po[step * DH * c + i];
+        }
+        const float inv = total == 0.f ? 0.f : 1.0f / total;
+        const uint32_t row = d.row0 + r, token = fastdiv(row, p.group), head = d.kvh * p.group.d + (row - token * p.group.d);
+        if (d.start >= p.b.nt || token >= p.b.nt - d.start) return;
+        elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(d.start + token) * p.o_st) + W * lane;
+#pragma unroll
+        for (int i = 0; i < W; ++i) dst[i] = f2e(out[i] * inv);
+    }
+}
+
+#define ATTN_PAGED(DH)                                                                                                                                   \
+    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_few_d##DH)(AttnPagedParams p) { attn_paged_few<DH>(p); }                  \
+    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH>(p); }                \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 16>(p); }           \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }
+ATTN_PAGED(64)
+ATTN_PAGED(128)
