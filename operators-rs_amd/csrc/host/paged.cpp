@@ -186,11 +186,15 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     const size_t steps = (m.cols * m.page + 31) / 32;
     a.min_steps = a.many ? 8 : 4;
     const size_t most = std::max<size_t>(1, steps / a.min_steps);
-    const size_t want = op && op->slots[a.many] > 0 ? (size_t)op->slots[a.many] : 2 * (size_t)(op ? op->dev->props.multiProcessorCount : 256);
+    // Key ranges for all tiles together: as many as workgroups of 128 rows run at a time (two per CU; 511 tokens over 32511
+    // keys, 32 heads over 8: 420 us with half as many, 321, 338 with twice as many), and twice that for 16 rows, where a range costs
+    // little and the rates of memory even out (50 decode steps over 165008 keys: 134 us with 512, 122 with 1024, 124 with 1536).
+    const size_t cus = (size_t)(op ? op->dev->props.multiProcessorCount : 256);
+    const size_t want = op && op->slots[a.many] > 0 ? (size_t)op->slots[a.many] : (a.many ? 2 : 4) * cus;
     a.grid = units;
     if (most > 1) {
-        a.slots = std::min(2 * want, units * most);
-        a.grid = std::min(units * most, units + 2 * want);
+        a.slots = std::min((4 * want + 2) / 3, units * most);
+        a.grid = std::min(units * most, units + (4 * want + 2) / 3);
         a.workspace = 64 + a.slots * (32 + tile * (m.dh + 2) * sizeof(float));
     }
     return a;
@@ -236,6 +240,9 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         Workspace ws(qa, workspace, workspace_len, plan.workspace);
         p.work = ws.ptr();
         p.slots = (uint32_t)plan.slots, p.min_steps = (uint32_t)plan.min_steps;
+        const ptrdiff_t far = (ptrdiff_t)1 << 31;
+        p.narrow = p.k_sp == p.v_sp && p.k_sr == p.v_sr && p.k_sp >= 0 && p.k_sp < far && p.k_sr >= 0 && p.k_sr < far / (ptrdiff_t)p.b.page.d &&
+                   p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;
         const int e = m.dt == OPHIP_DT_BF16, h = dh == 128;
         op->dev->make_current();
         launch(op->rows[e][plan.many][h], Dim3{(unsigned)plan.grid}, Dim3{256}, 0, stream_of(qa), p);
@@ -469,14 +476,16 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     const size_t vectors = dh * unit / 16;
     vec = vec && vectors <= 64;
     const int li = vectors <= 8 ? 0 : vectors <= 16 ? 1 : vectors <= 32 ? 2 : 3;
-    // few tokens: a token's heads over several workgroups, down to one row for each group of lanes
-    const size_t rows = vec ? 32u >> li : 4;
-    const size_t by = std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt));
-    p.heads_per_block = (uint32_t)((heads + by - 1) / by);
+    // Few tokens: a token's heads over several workgroups, down to one row for each group of lanes.  Many: several tokens to
+    // a workgroup, so that each of its 256 threads has one pair's sine and cosine to evaluate.
+    const size_t rows = vec ? 32u >> li : 4, tokens = vec && nt >= 4096 ? std::max<size_t>(1, 512 / dh) : 1;
+    const size_t by = tokens > 1 ? 1 : std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt)), per = (heads + by - 1) / by;
+    p.heads_per_block = make_fastdiv((uint32_t)per);
+    p.tokens_per_block = (uint32_t)tokens;
     op->dev->make_current();
     const int t = type_index(m.dt);
-    launch(vec ? op->vec[t][li] : op->pairs[t], Dim3{(unsigned)nt, (unsigned)((heads + p.heads_per_block - 1) / p.heads_per_block)}, Dim3{256},
-           p.rotate ? dh / 2 * 8 : 0, stream_of(qa), p);
+    launch(vec ? op->vec[t][li] : op->pairs[t], Dim3{(unsigned)((nt + tokens - 1) / tokens), (unsigned)((heads + per - 1) / per)}, Dim3{256},
+           p.rotate ? tokens * (dh / 2) * 8 : 0, stream_of(qa), p);
 }
 
 }  // namespace

@@ -18,12 +18,16 @@
 #include "paged.h"
 
 constexpr float PA_LOG2E = 1.4426950408889634f;
-// Probabilities are kept times 2^PA_BIAS (as are their sums): in f16, 2^-25 steps below 2^-14 would cost the many small
-// ones of a long row their bits.
+// The softmax is taken against a reference that trails the running maximum by at most 2^PA_LAG: sums and output are
+// rescaled only when a row's maximum has outgrown its reference by more, which after the first tiles is next to never (the
+// largest score of a row of random ones grows by its logarithm), instead of in most tiles (any of 32 rows will do).
+constexpr float PA_LAG = 8.f;
+// Probabilities are kept times 2^PA_BIAS (as are their sums), up to 2^15 with the lag: in f16, steps of 2^-24 below 2^-14
+// would cost the many small ones of a long row their bits.
 #ifdef GEMM_ELEM_BF16
 constexpr float PA_BIAS = 0.f;
 #else
-constexpr float PA_BIAS = 15.f;
+constexpr float PA_BIAS = 7.f;
 #endif
 
 // ---- the workspace: a count, a descriptor per slot (32 bytes), then per slot ROWS pairs (maximum, sum), then per slot
@@ -61,8 +65,8 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         if (lane == 0) s_work[wave] = work;
         __syncthreads();
         work = s_work[0] + s_work[1] + s_work[2] + s_work[3];
-        // half the slots: a count rounded up from more than one is less than twice as much
-        if (work) per_step = 0.4999995f * (float)p.slots / ((float)work * (float)p.nkvh);
+        // three quarters of the slots: a count rounded to two or more is at most four thirds of what it was
+        if (work) per_step = 0.749999f * (float)p.slots / ((float)work * (float)p.nkvh);
     } else __syncthreads();
     uint32_t items0 = 0, slots0 = 0;
     for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += 256) {
@@ -70,7 +74,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         if (i0 + tid < p.b.nseq) {
             const PagedSeq s = paged_seq(p.b, i0 + tid);
             const uint32_t most = steps_of(s) / p.min_steps;
-            if (p.slots && most > 1) pieces = min(most, max(1u, (uint32_t)ceilf((float)steps_of(s) * per_step)));
+            if (p.slots && most > 1) pieces = min(most, max(1u, (uint32_t)((float)steps_of(s) * per_step + 0.5f)));
             items = tiles_of(s) * p.nkvh * pieces;
             slots = pieces > 1 ? items : 0;
         }
@@ -176,7 +180,7 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
             pg[c] = min(page[c], p.b.npages - 1);
             const char *src = kb + (int64_t)pg[c] * p.k_sp + (int64_t)line[c] * p.k_sr;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) t.k[c][s] = ld128(src + 64 * s);
+            for (int s = 0; s < KS; ++s) t.k[c][s] = ld128_nt(src + 64 * s);
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -184,8 +188,8 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
             for (int i = 0; i < 4; ++i) {
                 const uint32_t vp = __shfl(pg[c], 4 * g + i, WAVE), vl = __shfl(line[c], 4 * g + i, WAVE);
                 const char *src = vb + (int64_t)vp * p.v_sp + (int64_t)vl * p.v_sr;
-                if constexpr (CW == 8) *reinterpret_cast<u32x4 *>(t.v[4 * c + i]) = ld128(src);
-                else *reinterpret_cast<u32x2 *>(t.v[4 * c + i]) = *reinterpret_cast<const u32x2 *>(src);
+                if constexpr (CW == 8) *reinterpret_cast<u32x4 *>(t.v[4 * c + i]) = ld128_nt(src);
+                else *reinterpret_cast<u32x2 *>(t.v[4 * c + i]) = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src));
             }
     };
     const float scale2 = p.scale * PA_LOG2E;
@@ -213,14 +217,14 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
         }
         mx = fmaxf(mx, __shfl_xor(mx, 16, WAVE));
         mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-        const float top = fmaxf(m, mx), ref = top == -INFINITY ? 0.f : top;
-        if (__builtin_amdgcn_ballot_w64(top != m) != 0) {
-            const float f = __builtin_amdgcn_exp2f(m - ref);
+        if (__builtin_amdgcn_ballot_w64(mx > m + PA_LAG) != 0) {
+            const float now = fmaxf(m, mx), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
             l *= f;
 #pragma unroll
             for (int c = 0; c < CW; ++c) o[c] *= f;
-            m = top;
+            m = now;
         }
+        const float ref = m == -INFINITY ? 0.f : m;
         PackE pr;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -244,6 +248,8 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
         look_up(first);
         fetch(a);
         look_up(first + 4);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) OPHIP_ARRIVED(q[s]);
         for (uint32_t step = first; step < last; step += 8) {
             if (step + 4 < last) {
                 fetch(b);
@@ -309,6 +315,11 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
 
 // ---- up to 128 rows: the products are the work
 //
+// Pages of a whole number of the rows that the workgroup loads at a time (RS) leave those rows in one page, so that the
+// page and the address are scalars and a thread adds an offset that never changes; in vector registers the same
+// arithmetic (products of 64 bits at a quarter of the rate) takes as long as the exponentials.  Other pages, caches that are
+// not alike and a tile that reaches past the last key take it row by row.
+//
 // A workgroup of four waves, 32 rows each, walks its key range in tiles of 64 keys that go through registers into LDS,
 // double-buffered, one barrier a tile; two workgroups share a CU.  S^T = K . Q^T with v_mfma 32x32x16: a lane holds one
 // query and half the tile's keys, so maxima, sums and factors are scalars of the lane; the probabilities are packed in
@@ -346,22 +357,50 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     const uint32_t cc = tid % CPR, cr = tid / CPR;
     const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 16 * cc;
     const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 16 * cc;
-    uint32_t line[NCH], page[NCH];
+    uint32_t page[NCH], line[NCH];  // of the next tile's rows: scalars when `aligned`
     u32x4 kreg[NCH], vreg[NCH];
+    const bool aligned = p.narrow && p.b.page.d % RS == 0;
+    const uint32_t off = cr * (uint32_t)p.k_sr + 16 * cc;
+    const char *kh = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh, *vh = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh;
+    const char *table = reinterpret_cast<const char *>(p.b.table) + (int64_t)it.seq * p.b.t_row;
     auto look_up = [&](uint32_t t) {
+        if (aligned) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const uint32_t key = min(t * BN + cr + RS * i, it.s.len - 1), col = fastdiv(key, p.b.page);
-            line[i] = key - col * p.b.page.d;
-            page[i] = paged_page(p.b, it.seq, col);
+            for (int i = 0; i < NCH; ++i) {
+                const uint32_t key = min(t * BN + RS * i, it.s.len - 1), col = fastdiv(key, p.b.page);
+                line[i] = key - col * p.b.page.d;
+                page[i] = *reinterpret_cast<const uint32_t *>(table + col * (uint32_t)p.b.t_col);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const uint32_t key = min(t * BN + cr + RS * i, it.s.len - 1), col = fastdiv(key, p.b.page);
+                line[i] = key - col * p.b.page.d;
+                page[i] = *reinterpret_cast<const uint32_t *>(table + (int64_t)col * p.b.t_col);
+            }
         }
     };
-    auto fetch = [&]() {
+    auto fetch = [&](uint32_t t) {
+        if (aligned && t * BN + BN <= it.s.len) {
 #pragma unroll
-        for (int i = 0; i < NCH; ++i) {
-            const uint32_t pg = min(page[i], p.b.npages - 1);
-            kreg[i] = ld128(kb + (int64_t)pg * p.k_sp + (int64_t)line[i] * p.k_sr);
-            vreg[i] = ld128(vb + (int64_t)pg * p.v_sp + (int64_t)line[i] * p.v_sr);
+            for (int i = 0; i < NCH; ++i) {
+                const uint32_t pg = __builtin_amdgcn_readfirstlane(min(page[i], p.b.npages - 1)), ln = __builtin_amdgcn_readfirstlane(line[i]);
+                const uint64_t at = (uint64_t)pg * (uint32_t)p.k_sp + ln * (uint32_t)p.k_sr;
+                kreg[i] = ld128(kh + at + off);
+                vreg[i] = ld128(vh + at + off);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NCH; ++i) {
+                const uint32_t pg = min(page[i], p.b.npages - 1);
+                uint32_t ln = line[i];
+                if (aligned) {  // the first of the RS rows, or the last key
+                    const uint32_t key = t * BN + RS * i;
+                    if (key < it.s.len) ln += min(cr, it.s.len - 1 - key);
+                }
+                kreg[i] = ld128(kb + (int64_t)pg * p.k_sp + (int64_t)ln * p.k_sr);
+                vreg[i] = ld128(vb + (int64_t)pg * p.v_sp + (int64_t)ln * p.v_sr);
+            }
         }
     };
     auto commit = [&](int buf) {
@@ -381,20 +420,23 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
 
     if (first < last) {
         look_up(first);
-        fetch();
+        fetch(first);
         commit(0);
         if (first + 1 < last) look_up(first + 1);
     }
+#pragma unroll
+    for (int d = 0; d < DS; ++d) OPHIP_ARRIVED(qf[d].u);
     __syncthreads();
     for (uint32_t t = first; t < last; ++t) {
         const int buf = (t - first) & 1;
         const bool more = t + 1 < last;
         if (more) {
-            fetch();
+            fetch(t + 1);
             look_up(t + 2);
         }
         if ((int32_t)(t * BN) < lim_last) {
             const elem *kt = k_lds[buf], *vt = v_lds[buf];
+            __builtin_amdgcn_s_setprio(1);
             // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
             f32x16 sacc[2];
 #pragma unroll
@@ -408,6 +450,7 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
                     sacc[b] = mfma_32x32x16(a.h, qf[d].h, sacc[b]);
                 }
             }
+            __builtin_amdgcn_s_setprio(0);
             if ((int32_t)(t * BN + BN) > lim_first) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -421,17 +464,17 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) mx = fmaxf(mx, sacc[b][e]);
             mx = fmaxf(mx, __shfl_xor(mx, 32, WAVE));
-            const float top = fmaxf(m, mx * scale2), ref = top == -INFINITY ? 0.f : top;
-            if (__builtin_amdgcn_ballot_w64(top != m) != 0) {
-                const float f = __builtin_amdgcn_exp2f(m - ref);
+            const float top = mx * scale2;
+            if (__builtin_amdgcn_ballot_w64(top > m + PA_LAG) != 0) {
+                const float now = fmaxf(m, top), f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
                 l *= f;
 #pragma unroll
                 for (int d = 0; d < DB; ++d)
 #pragma unroll
                     for (int e = 0; e < 16; ++e) o[d][e] *= f;
-                m = top;
+                m = now;
             }
-            const float shift = PA_BIAS - ref;
+            const float shift = PA_BIAS - (m == -INFINITY ? 0.f : m);  // (a row that has kept nothing so far: every term is 0)
             float sum = 0.f;
             PackE pb[4];  // MFMA n: the tile's keys 16 n .. + 15, slots 8 h .. 8 h + 7 keys 16 n + 4 h + {0..3}, 16 n + 8 + 4 h + {0..3}
 #pragma unroll
@@ -444,6 +487,7 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
                 }
             l += sum;
             typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -458,6 +502,7 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
                     o[d] = mfma_32x32x16(a.hv, pb[n].h, o[d]);
                 }
         }
+        __builtin_amdgcn_s_setprio(0);
         if (more) commit(buf ^ 1);
         __syncthreads();
     }

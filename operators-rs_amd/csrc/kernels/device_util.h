@@ -37,6 +37,14 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 #define OPHIP_WAVE_LOCKSTEP() ((void)0)
 #endif
 
+// The value is in its registers from here on.  In front of a loop that uses what was loaded before it: without, the compiler
+// waits for the load at its first use inside the loop, in every round, and so for whatever that round has requested since.
+#ifdef OPHIP_CPU_SIM
+#define OPHIP_ARRIVED(x) ((void)0)
+#else
+#define OPHIP_ARRIVED(x) asm volatile("" : "+v"(x))
+#endif
+
 // Threads per workgroup of every kernel that strides by its workgroup size (the host launches them with exactly this
 // many).  A constant rather than blockDim.x: inside a __device__ function the compiler fetches blockDim.x with a vector
 // load from the implicit arguments and waits for it before the first address is known, which costs a streaming kernel of

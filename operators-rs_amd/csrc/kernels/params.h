@@ -289,6 +289,7 @@ struct AttnPagedParams {
     FastDivU32 group;  // query heads per kv head
     uint32_t nkvh, dh, causal;
     uint32_t slots;     // key ranges the work area holds, and the number that the tiles are split into together; 0: no splitting
+    uint32_t narrow;  // both caches of one layout, and distances inside a page, a row of the table and from page to page of less than 32 bits
     uint32_t min_steps;  // a range has at least this many steps of 32 keys
     float scale;
 };
@@ -310,9 +311,9 @@ struct QkNormRopeParams {
     void *y[2];
     int64_t x_st[2], x_sh[2], y_st[2], y_sh[2], p_step;
     uint32_t nt, nh[2], dh;
-    uint32_t heads_per_block;  // of the nh[0] + nh[1] heads of a token
+    struct FastDivU32 heads_per_block;  // of the nh[0] + nh[1] heads of a token; all of them where tokens_per_block > 1
+    uint32_t tokens_per_block;
     uint32_t pos_is_u64, rotate, w_is_f32;
     float epsilon;
-    uint32_t _pad;
     double freq_step;  // log2(theta) / (dh / 2)
 };

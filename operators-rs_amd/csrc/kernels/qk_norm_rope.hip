@@ -1,60 +1,92 @@
 // qk_norm_rope: y = rope(x / sqrt(mean(x^2) + epsilon) * w, p) for every head of q and of k, in one pass and one launch.
 //
-// A workgroup serves one token, or one slice of its nh + nkh heads: its sines and cosines are evaluated once into LDS
-// while the first rows travel.  A row (one head) is 16 bytes in each of L consecutive lanes, so its sum of squares is a
-// sum over L lanes and everything else stays in the lane: each byte is read once and written once.
+// A workgroup serves some consecutive tokens, or one slice of one token's nh + nkh heads when there are few.  A row (one
+// head) is 16 bytes in each of L consecutive lanes, so its sum of squares is a sum over L lanes and everything else stays
+// in the lane: each byte is read once and written once, and what bounds the kernel is memory.  The tokens' sines and
+// cosines are evaluated once into LDS, a pair of a token per thread, while the first rows travel: 256 / (dh / 2) tokens
+// give every thread one (an evaluation is some fifty f64 instructions; a token per workgroup leaves three
+// quarters of the threads of dh 128 waiting for it: 65 us against 45 for 8191 tokens of 40 heads), and four rows per
+// thread are on their way at a time.
 #include "paged.h"
 
-extern __shared__ float2 qk_sc[];  // dh / 2 entries of (sin, cos)
+extern __shared__ float2 qk_sc[];  // [token][dh / 2] of (sin, cos)
 
-__device__ __forceinline__ void qk_fill_table(const QkNormRopeParams &p, uint32_t token) {
-    const double pos = rope_position(p.pos, (int64_t)token * p.p_step, p.pos_is_u64);
-    for (uint32_t k = threadIdx.x; k < p.dh / 2; k += WG_THREADS) qk_sc[k] = rope_sin_cos(pos, rope_turns(p.freq_step, k));
+__device__ __forceinline__ void qk_fill_table(const QkNormRopeParams &p, uint32_t token0, uint32_t tokens) {
+    const uint32_t half = p.dh / 2;
+    for (uint32_t e = threadIdx.x; e < tokens * half; e += WG_THREADS) {
+        const uint32_t t = e / half;
+        qk_sc[e] = rope_sin_cos(rope_position(p.pos, (int64_t)(token0 + t) * p.p_step, p.pos_is_u64), rope_turns(p.freq_step, e - t * half));
+    }
+    __syncthreads();
 }
 
 // Rows of whole 16-byte vectors, aligned; L = the power of two of lanes that holds one (lanes past dh idle)
 template <typename T, int L>
 __device__ __forceinline__ void qk_norm_rope_vec(const QkNormRopeParams &p) {
-    constexpr int E = 16 / sizeof(T);
-    const uint32_t token = blockIdx.x, lane = threadIdx.x % L;
-    const uint32_t h0 = blockIdx.y * p.heads_per_block, h1 = min(h0 + p.heads_per_block, p.nh[0] + p.nh[1]);
+    constexpr int E = 16 / sizeof(T), G = WG_THREADS / L, U = 4;
+    const uint32_t token0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.nt - token0), lane = threadIdx.x % L;
+    const uint32_t heads = p.heads_per_block.d, h0 = blockIdx.y * heads, h1 = p.nh[0] + p.nh[1], rows = tokens * heads;
     const bool live = lane * E < p.dh;
-    if (p.rotate) {
-        qk_fill_table(p, token);
-        __syncthreads();
-    }
-    for (uint32_t h = h0 + threadIdx.x / L; h < h1; h += WG_THREADS / L) {
-        const uint32_t which = h >= p.nh[0], hh = which ? h - p.nh[0] : h;
-        PackOf<T> x;
-        x.u = u32x4{0, 0, 0, 0};
-        if (live) x.u = ld128(reinterpret_cast<const char *>(p.x[which]) + (int64_t)token * p.x_st[which] + (int64_t)hh * p.x_sh[which] + 16 * lane);
-        float f[E], sum = 0.f;
+    float w[2][E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) {
-            f[i] = (float)x.e[i];
-            sum += f[i] * f[i];
+    for (int i = 0; i < E; ++i) w[0][i] = w[1][i] = 0.f;
+    auto weights = [&]() {
+        if (!live) return;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if (p.nh[k] == 0) continue;
+#pragma unroll
+            for (int i = 0; i < E; ++i)
+                w[k][i] = p.w_is_f32 ? reinterpret_cast<const float *>(p.w[k])[lane * E + i] : (float)reinterpret_cast<const T *>(p.w[k])[lane * E + i];
+        }
+    };
+    bool first = true;
+    for (uint32_t r0 = threadIdx.x / L; first || r0 < rows; r0 += U * G) {
+        PackOf<T> x[U];
+        uint32_t tok[U], which[U], head[U];
+        bool on[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t r = r0 + u * G;
+            tok[u] = fastdiv(r, p.heads_per_block);
+            const uint32_t h = h0 + r - tok[u] * heads;
+            on[u] = live && r < rows && h < h1;
+            which[u] = h >= p.nh[0];
+            head[u] = which[u] ? h - p.nh[0] : h;
+            x[u].u = u32x4{0, 0, 0, 0};
+            if (on[u]) x[u].u = ld128(reinterpret_cast<const char *>(p.x[which[u]]) + (int64_t)(token0 + tok[u]) * p.x_st[which[u]] + (int64_t)head[u] * p.x_sh[which[u]] + 16 * lane);
+        }
+        if (first) {  // (the same for the whole workgroup)
+            weights();
+            if (p.rotate) qk_fill_table(p, token0, tokens);
+            first = false;
         }
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
-        const float r = rsqrtf(sum / (float)p.dh + p.epsilon);
-        if (live) {
+        for (int u = 0; u < U; ++u) {
+            float f[E], sum = 0.f;
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const uint32_t e = lane * E + i;
-                f[i] *= r * (p.w_is_f32 ? reinterpret_cast<const float *>(p.w[which])[e] : (float)reinterpret_cast<const T *>(p.w[which])[e]);
+                f[i] = (float)x[u].e[i];
+                sum += f[i] * f[i];
             }
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) sum += __shfl_xor(sum, o, WAVE);
+            if (!on[u]) continue;
+            const float r = rsqrtf(sum / (float)p.dh + p.epsilon);
+#pragma unroll
+            for (int i = 0; i < E; ++i) f[i] *= r * (which[u] ? w[1][i] : w[0][i]);
             if (p.rotate) {
+                const float2 *sc = qk_sc + tok[u] * (p.dh / 2) + lane * (E / 2);
 #pragma unroll
                 for (int i = 0; i < E / 2; ++i) {
-                    const float2 sc = qk_sc[lane * (E / 2) + i];
                     const float a = f[2 * i], b = f[2 * i + 1];
-                    f[2 * i] = a * sc.y - b * sc.x;
-                    f[2 * i + 1] = a * sc.x + b * sc.y;
+                    f[2 * i] = a * sc[i].y - b * sc[i].x;
+                    f[2 * i + 1] = a * sc[i].x + b * sc[i].y;
                 }
             }
 #pragma unroll
-            for (int i = 0; i < E; ++i) x.e[i] = (T)f[i];
-            st128(reinterpret_cast<char *>(p.y[which]) + (int64_t)token * p.y_st[which] + (int64_t)hh * p.y_sh[which] + 16 * lane, x.u);
+            for (int i = 0; i < E; ++i) x[u].e[i] = (T)f[i];
+            st128(reinterpret_cast<char *>(p.y[which[u]]) + (int64_t)(token0 + tok[u]) * p.y_st[which[u]] + (int64_t)head[u] * p.y_sh[which[u]] + 16 * lane, x[u].u);
         }
     }
 }
@@ -63,11 +95,8 @@ __device__ __forceinline__ void qk_norm_rope_vec(const QkNormRopeParams &p) {
 template <typename T>
 __device__ __forceinline__ void qk_norm_rope_pairs(const QkNormRopeParams &p) {
     const uint32_t token = blockIdx.x, lane = threadIdx.x % WAVE;
-    const uint32_t h0 = blockIdx.y * p.heads_per_block, h1 = min(h0 + p.heads_per_block, p.nh[0] + p.nh[1]);
-    if (p.rotate) {
-        qk_fill_table(p, token);
-        __syncthreads();
-    }
+    const uint32_t h0 = blockIdx.y * p.heads_per_block.d, h1 = min(h0 + p.heads_per_block.d, p.nh[0] + p.nh[1]);
+    if (p.rotate) qk_fill_table(p, token, 1);
     for (uint32_t h = h0 + threadIdx.x / WAVE; h < h1; h += WG_THREADS / WAVE) {
         const uint32_t which = h >= p.nh[0], hh = which ? h - p.nh[0] : h;
         const T *x = reinterpret_cast<const T *>(reinterpret_cast<const char *>(p.x[which]) + (int64_t)token * p.x_st[which] + (int64_t)hh * p.x_sh[which]);

@@ -534,6 +534,9 @@ class _Operator:
         h = ctypes.c_void_p()
         _check(getattr(lib(), "ophip_%s_create" % self.NAME)(node.handle, ctypes.byref(h)))
         self.handle = h
+        # (a function object of its own: declared argument types convert faster than objects made for each call)
+        self._launch = lib()["ophip_%s_launch" % self.NAME]
+        self._launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
 
     def scheme(self, args, max_workspace_size=0):
         ws = ctypes.c_size_t(0)
@@ -546,11 +549,12 @@ class _Operator:
         if workspace is None:
             wp, wl = None, 0
         elif isinstance(workspace, DevMem):
-            wp, wl = ctypes.c_void_p(workspace.ptr), workspace.size
+            wp, wl = workspace.ptr, workspace.size
         else:
-            wp, wl = ctypes.c_void_p(workspace[0]), workspace[1]
-        _check(getattr(lib(), "ophip_%s_launch" % self.NAME)(self.handle, ctypes.byref(args.c()), wp,
-                                                             ctypes.c_size_t(wl), _qa(queue_alloc)), launch=True)
+            wp, wl = workspace
+        code = self._launch(self.handle, ctypes.byref(args.c()), wp, wl, _qa(queue_alloc))
+        if code:
+            _check(code, launch=True)
 
     def destroy(self):
         if self.handle is not None:
@@ -725,7 +729,24 @@ class AttnKVCachedArgs:
                                  DYN_USIZE if self.pos is None else self.pos)
 
 
-class AttentionPagedArgs:
+class _KeptArgs:
+    """Arguments that a serving loop launches again and again: the C struct is made at the first launch and kept until an
+    attribute is set.  Only where every base is a plain address: a DevMem is asked for its own each time."""
+
+    def __setattr__(self, name, value):
+        self.__dict__.pop("_struct", None)
+        self.__dict__[name] = value
+
+    def c(self):
+        kept = self.__dict__.get("_struct")
+        if kept is None:
+            kept = self._make()
+            if not any(isinstance(v, DevMem) for v in self.__dict__.values()):
+                self.__dict__["_struct"] = kept
+        return kept
+
+
+class AttentionPagedArgs(_KeptArgs):
     """attention over a paged cache; the layouts are described in include/ophip.h"""
 
     def __init__(self, q_layout, q_base, k_cache_layout, k_cache_base, v_cache_layout, v_cache_base, o_layout,
@@ -733,7 +754,7 @@ class AttentionPagedArgs:
                  kv_len_base, mask, scale):
         self.__dict__.update(locals())
 
-    def c(self):
+    def _make(self):
         return _AttentionPagedArgs(self.q_layout.c(), _p(self.q_base), self.k_cache_layout.c(),
                                     _p(self.k_cache_base), self.v_cache_layout.c(), _p(self.v_cache_base),
                                     self.o_layout.c(), _p(self.o_base), self.page_table_layout.c(),
@@ -741,7 +762,7 @@ class AttentionPagedArgs:
                                     self.kv_len_layout.c(), _p(self.kv_len_base), self.mask, self.scale)
 
 
-class KvAppendPagedArgs:
+class KvAppendPagedArgs(_KeptArgs):
     """k and v into a paged cache, k rotated on the way (theta = 0: not)"""
 
     def __init__(self, k_layout, k_base, v_layout, v_base, p_layout, p_base, k_cache_layout, k_cache_base,
@@ -749,7 +770,7 @@ class KvAppendPagedArgs:
                  q_start_base, kv_len_layout, kv_len_base, theta):
         self.__dict__.update(locals())
 
-    def c(self):
+    def _make(self):
         return _KvAppendPagedArgs(self.k_layout.c(), _p(self.k_base), self.v_layout.c(), _p(self.v_base),
                                    self.p_layout.c(), _p(self.p_base), self.k_cache_layout.c(),
                                    _p(self.k_cache_base), self.v_cache_layout.c(), _p(self.v_cache_base),
@@ -758,14 +779,14 @@ class KvAppendPagedArgs:
                                    _p(self.kv_len_base), self.theta)
 
 
-class QkNormRopeArgs:
+class QkNormRopeArgs(_KeptArgs):
     """rms_norm of every query and key head, then rope (theta = 0: the norms alone)"""
 
     def __init__(self, qy_layout, qy_base, q_layout, q_base, qw_layout, qw_base, ky_layout, ky_base, k_layout,
                  k_base, kw_layout, kw_base, p_layout, p_base, epsilon, theta):
         self.__dict__.update(locals())
 
-    def c(self):
+    def _make(self):
         return _QkNormRopeArgs(self.qy_layout.c(), _p(self.qy_base), self.q_layout.c(), _p(self.q_base),
                                 self.qw_layout.c(), _p(self.qw_base), self.ky_layout.c(), _p(self.ky_base),
                                 self.k_layout.c(), _p(self.k_base), self.kw_layout.c(), _p(self.kw_base),
