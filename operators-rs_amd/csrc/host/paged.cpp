@@ -167,7 +167,7 @@ AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
 struct AttnPagedPlan {
     bool matrix;                    // they serve these types and sizes
     int many;                       // tiles of 128 rows, or of 16
-    size_t grid, slots, min_steps;  // workgroups; key ranges the workspace holds (0: no tile can be cut); steps of 32 keys a range has at least
+    size_t grid, slots;  // workgroups; key ranges the workspace holds (0: no tile can be cut)
     size_t workspace;
 };
 AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPagedMeta &m) {
@@ -184,8 +184,7 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     // the most tiles there can be, whatever the lengths: each sequence that has a token may have one that is not full
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
     const size_t steps = (m.cols * m.page + 31) / 32;
-    a.min_steps = a.many ? 8 : 4;
-    const size_t most = std::max<size_t>(1, steps / a.min_steps);
+    const size_t most = std::max<size_t>(1, steps / 4);  // (a key range has four steps of 32 keys at least)
     // Key ranges for all tiles together: as many as workgroups of 128 rows run at a time (two per CU; 511 tokens over 32511
     // keys, 32 heads over 8: 420 us with half as many, 321, 338 with twice as many), and twice that for 16 rows, where a range costs
     // little and the rates of memory even out (50 decode steps over 165008 keys: 134 us with 512, 122 with 1024, 124 with 1536).
@@ -239,7 +238,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base)) {
         Workspace ws(qa, workspace, workspace_len, plan.workspace);
         p.work = ws.ptr();
-        p.slots = (uint32_t)plan.slots, p.min_steps = (uint32_t)plan.min_steps;
+        p.slots = (uint32_t)plan.slots;
         const ptrdiff_t far = (ptrdiff_t)1 << 31;
         p.narrow = p.k_sp == p.v_sp && p.k_sr == p.v_sr && p.k_sp >= 0 && p.k_sp < far && p.k_sr >= 0 && p.k_sr < far / (ptrdiff_t)p.b.page.d &&
                    p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;

@@ -2,16 +2,19 @@
 // unlike lengths, f16 / bf16, dh 64 and 128.
 //
 // Work units.  The query rows of one kv head and sequence are its new tokens times the `group` query heads that share
-// the kv head, row = token * group + head-in-group, cut into tiles of 16 rows (attn_paged_few: decode steps, where the
-// caches are all the traffic) or 128 (attn_paged_many: prompts and chunks, where the products are the work).  So keys and
-// values are read once per tile whatever the group, and a short group fills the rows with further tokens.
+// the kv head, row = token * group + head-in-group.  A sequence of up to 16 rows (a decode step) is one tile that
+// paged_few works on: the caches are all the traffic.  One of more rows (prompts, chunks) is cut into tiles of 128 rows for
+// paged_many: the products are the work.  So keys and values are read once per tile whatever the group, and a short
+// group fills the rows with further tokens.  Two kernels: attn_paged_few, on tiles of 16 rows only, for batches that are
+// nearly all decode steps, and attn_paged_many, which has both inside and gives each sequence its own (25 sequences
+// over 56185 keys, one of them a chunk of 333 tokens, dh 64: 36 us with all of them on tiles of 128 rows, BOTH with both).
 //
 // Plan.  The host knows the number of tokens and sequences, not the lengths, and must not wait for them; so every
-// workgroup works its own unit out from the lengths on the device (paged_item: two prefix sums over the sequences, about a
-// microsecond): the tiles of a sequence with more keys than 1 / slots of all tiles' keys are cut into that many more
-// key ranges, one workgroup each, so that a launch has about `slots` equal pieces of work whatever the mix of lengths.
-// Ranges of a cut tile leave their maximum, sum and output in the workspace and attn_paged_join merges them in a fixed
-// order: results do not depend on which workgroup ends first.
+// workgroup works its own unit out from the lengths on the device (paged_item: a prefix sum over the sequences).  The tiles
+// of a sequence with more keys than 1 / slots of all tiles' keys are cut into that many more key ranges, one workgroup
+// each, so that a launch has about `slots` equal pieces of work whatever the mix of lengths.  Ranges of a cut tile leave
+// their maximum, sum and output in the workspace and attn_paged_join merges them in a fixed order: results do not
+// depend on which workgroup ends first.
 //
 // Compiled twice, like the other MFMA kernels (gemm_elem.h).
 #include "gemm_elem.h"
@@ -45,73 +48,119 @@ struct PagedItem {
     uint32_t row0, nrows;                     // rows of the sequence and kv head
 };
 
-// What workgroup blockIdx.x does; false: nothing.  Every thread of the 256 or more calls it and gets the same.
+constexpr uint32_t FEW = 16;
+template <int ROWS>
+__device__ __forceinline__ uint32_t paged_tiles(const AttnPagedParams &p, const PagedSeq &s) {
+    const uint64_t rows = (uint64_t)s.n * p.group.d;
+    return rows <= FEW ? (rows ? 1 : 0) : (uint32_t)((rows + ROWS - 1) / ROWS);
+}
+__device__ __forceinline__ uint32_t paged_steps(const PagedSeq &s) { return (s.len + 31) / 32; }
+// Key ranges that a sequence's tiles are cut into, from the ranges that a step of 32 keys is worth
+template <int ROWS>
+__device__ __forceinline__ uint32_t paged_pieces(const AttnPagedParams &p, const PagedSeq &s, float per_step) {
+    const uint32_t least = (uint64_t)s.n * p.group.d <= FEW ? 4 : 8;  // steps in a range: one for each wave, four tiles of 64 keys
+    const uint32_t most = paged_steps(s) / least;
+    return p.slots && most > 1 ? min(most, max(1u, (uint32_t)((float)paged_steps(s) * per_step + 0.5f))) : 1;
+}
+// `work`: tiles times steps of all sequences.  Three quarters of the slots: a count rounded to two or more is at most four
+// thirds of what it was.
+__device__ __forceinline__ float paged_per_step(const AttnPagedParams &p, float work) {
+    return work > 0.f ? 0.74999f * (float)p.slots / (work * (float)p.nkvh) : 0.f;
+}
+
+// What workgroup blockIdx.x does; false: nothing.  Every thread calls it and gets the same.
 template <int ROWS>
 __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &it) {
-    __shared__ uint64_t s_work[4];
-    __shared__ uint32_t s_scan[2][4], s_found[4];
     const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE, w = blockIdx.x;
-    auto tiles_of = [&](const PagedSeq &s) { return (uint32_t)(((uint64_t)s.n * p.group.d + ROWS - 1) / ROWS); };
-    auto steps_of = [&](const PagedSeq &s) { return (s.len + 31) / 32; };
-    float per_step = 0.f;  // key ranges per step of 32 keys
-    if (tid == 0) s_found[0] = 0xffffffffu;
-    if (p.slots) {
-        uint64_t work = 0;
-        for (uint32_t i = tid; i < p.b.nseq; i += 256) {
-            const PagedSeq s = paged_seq(p.b, i);
-            work += (uint64_t)tiles_of(s) * steps_of(s);
+    uint32_t local, first_slot;
+    if (p.b.nseq <= WAVE) {
+        // A sequence per lane, each wave for itself.  The longest come first: the units that end last should not also
+        // begin last.
+        const bool on = lane < p.b.nseq;
+        PagedSeq s{0, 0, 0};
+        if (on) s = paged_seq(p.b, lane);
+        const uint32_t tiles = paged_tiles<ROWS>(p, s);
+        const float work = p.slots ? wave_sum_dpp((float)tiles * (float)paged_steps(s)) : 0.f;
+        const uint32_t pieces = paged_pieces<ROWS>(p, s, paged_per_step(p, work));
+        const uint32_t items = tiles * p.nkvh * pieces, slots = pieces > 1 ? items : 0;
+        uint32_t items0 = 0, slots0 = 0, all_slots = 0;
+        for (uint32_t k = 0; k < p.b.nseq; ++k) {
+            const uint32_t len = __builtin_amdgcn_readlane(s.len, k), ni = __builtin_amdgcn_readlane(items, k), ns = __builtin_amdgcn_readlane(slots, k);
+            const bool before = len > s.len || (len == s.len && k < lane);
+            items0 += before ? ni : 0;
+            slots0 += before ? ns : 0;
+            all_slots += ns;
         }
-        work = wave_sum(work);
-        if (lane == 0) s_work[wave] = work;
+        if (w == 0 && tid == 0 && p.slots) *reinterpret_cast<uint32_t *>(p.work) = min(all_slots, p.slots);
+        const uint64_t mine = __builtin_amdgcn_ballot_w64(w - items0 < items);
+        if (mine == 0) return false;
+        const uint32_t at = (uint32_t)__ffsll((long long)mine) - 1;
+        it.seq = at;
+        it.s = PagedSeq{(uint32_t)__builtin_amdgcn_readlane(s.start, at), (uint32_t)__builtin_amdgcn_readlane(s.n, at), (uint32_t)__builtin_amdgcn_readlane(s.len, at)};
+        it.pieces = __builtin_amdgcn_readlane(pieces, at);
+        local = w - __builtin_amdgcn_readlane(items0, at);
+        first_slot = __builtin_amdgcn_readlane(slots0, at);
+    } else {
+        __shared__ float s_work[4];
+        __shared__ uint32_t s_scan[2][4], s_found[4];
+        float per_step = 0.f;
+        if (tid == 0) s_found[0] = 0xffffffffu;
+        if (p.slots) {
+            float work = 0.f;
+            for (uint32_t i = tid; i < p.b.nseq; i += 256) {
+                const PagedSeq s = paged_seq(p.b, i);
+                work += (float)paged_tiles<ROWS>(p, s) * (float)paged_steps(s);
+            }
+            work = wave_sum_dpp(work);
+            if (lane == 0) s_work[wave] = work;
+        }
         __syncthreads();
-        work = s_work[0] + s_work[1] + s_work[2] + s_work[3];
-        // three quarters of the slots: a count rounded to two or more is at most four thirds of what it was
-        if (work) per_step = 0.749999f * (float)p.slots / ((float)work * (float)p.nkvh);
-    } else __syncthreads();
-    uint32_t items0 = 0, slots0 = 0;
-    for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += 256) {
-        uint32_t items = 0, slots = 0, pieces = 1;
-        if (i0 + tid < p.b.nseq) {
-            const PagedSeq s = paged_seq(p.b, i0 + tid);
-            const uint32_t most = steps_of(s) / p.min_steps;
-            if (p.slots && most > 1) pieces = min(most, max(1u, (uint32_t)((float)steps_of(s) * per_step + 0.5f)));
-            items = tiles_of(s) * p.nkvh * pieces;
-            slots = pieces > 1 ? items : 0;
-        }
-        uint32_t a = items, b = slots;
+        if (p.slots) per_step = paged_per_step(p, s_work[0] + s_work[1] + s_work[2] + s_work[3]);
+        uint32_t items0 = 0, slots0 = 0;
+        for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += 256) {
+            uint32_t items = 0, slots = 0, pieces = 1;
+            if (i0 + tid < p.b.nseq) {
+                const PagedSeq s = paged_seq(p.b, i0 + tid);
+                pieces = paged_pieces<ROWS>(p, s, per_step);
+                items = paged_tiles<ROWS>(p, s) * p.nkvh * pieces;
+                slots = pieces > 1 ? items : 0;
+            }
+            uint32_t a = items, b = slots;
 #pragma unroll
-        for (int o = 1; o < WAVE; o <<= 1) {
-            const uint32_t ua = __shfl_up(a, o, WAVE), ub = __shfl_up(b, o, WAVE);
-            if (lane >= (uint32_t)o) a += ua, b += ub;
-        }
-        if (lane == WAVE - 1) s_scan[0][wave] = a, s_scan[1][wave] = b;
-        __syncthreads();
-        uint32_t ta = 0, tb = 0;
+            for (int o = 1; o < WAVE; o <<= 1) {
+                const uint32_t ua = __shfl_up(a, o, WAVE), ub = __shfl_up(b, o, WAVE);
+                if (lane >= (uint32_t)o) a += ua, b += ub;
+            }
+            if (lane == WAVE - 1) s_scan[0][wave] = a, s_scan[1][wave] = b;
+            __syncthreads();
+            uint32_t ta = 0, tb = 0;
 #pragma unroll
-        for (uint32_t v = 0; v < 4; ++v) {
-            if (v < wave) a += s_scan[0][v], b += s_scan[1][v];
-            ta += s_scan[0][v], tb += s_scan[1][v];
+            for (uint32_t v = 0; v < 4; ++v) {
+                if (v < wave) a += s_scan[0][v], b += s_scan[1][v];
+                ta += s_scan[0][v], tb += s_scan[1][v];
+            }
+            const uint32_t before = items0 + a - items;
+            if (w - before < items) s_found[0] = i0 + tid, s_found[1] = w - before, s_found[2] = pieces, s_found[3] = slots0 + b - slots;
+            items0 += ta, slots0 += tb;
+            __syncthreads();
+            if (w < items0 && w != 0) break;  // (workgroup 0 counts all slots)
         }
-        const uint32_t before = items0 + a - items;
-        if (w - before < items) s_found[0] = i0 + tid, s_found[1] = w - before, s_found[2] = pieces, s_found[3] = slots0 + b - slots;
-        items0 += ta, slots0 += tb;
-        __syncthreads();
-        if (w < items0 && w != 0) break;  // (workgroup 0 counts all slots)
+        if (w == 0 && tid == 0 && p.slots) *reinterpret_cast<uint32_t *>(p.work) = min(slots0, p.slots);
+        if (s_found[0] == 0xffffffffu) return false;
+        it.seq = __builtin_amdgcn_readfirstlane(s_found[0]);
+        local = __builtin_amdgcn_readfirstlane(s_found[1]);
+        it.pieces = __builtin_amdgcn_readfirstlane(s_found[2]);
+        first_slot = __builtin_amdgcn_readfirstlane(s_found[3]);
+        it.s = paged_seq(p.b, it.seq);
     }
-    if (w == 0 && tid == 0 && p.slots) *reinterpret_cast<uint32_t *>(p.work) = min(slots0, p.slots);
-    if (s_found[0] == 0xffffffffu) return false;
-    it.seq = __builtin_amdgcn_readfirstlane(s_found[0]);
-    const uint32_t local = __builtin_amdgcn_readfirstlane(s_found[1]);
-    it.pieces = __builtin_amdgcn_readfirstlane(s_found[2]);
-    it.slot = __builtin_amdgcn_readfirstlane(s_found[3]) + local;
+    it.slot = first_slot + local;
     if (it.pieces > 1 && it.slot >= p.slots) return false;
-    it.s = paged_seq(p.b, it.seq);
     // kv heads next to each other (consecutive workgroups go to different XCDs, so a kv head's tiles meet in one L2), a
     // tile's ranges next, the tiles last to first: the last has the most keys under a causal mask
     it.kvh = local % p.nkvh;
-    const uint32_t rest = local / p.nkvh, rows = it.s.n * p.group.d, back = rest / it.pieces;
+    const uint32_t rest = local / p.nkvh, rows = it.s.n * p.group.d, back = rest / it.pieces, tiles = paged_tiles<ROWS>(p, it.s);
     it.piece = rest - back * it.pieces;
-    it.row0 = (tiles_of(it.s) - 1 - back) * ROWS;
+    it.row0 = (tiles - 1 - back) * ROWS;
     it.nrows = min((uint32_t)ROWS, rows - it.row0);
     if (it.pieces > 1 && tid == 0) paged_desc(p)[it.slot] = PagedDesc{it.piece, it.pieces, it.kvh, it.row0, it.nrows, it.s.start, {0, 0}};
     return true;
@@ -143,11 +192,14 @@ struct FewTile {  // 32 keys
 };
 
 template <int DH>
-__device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
+struct FewLds {
+    float m[4][16], l[4][16], o[4][DH / 4][WAVE];
+};
+
+// ROWS: of the tiles whose partial results the workspace holds
+template <int DH, int ROWS>
+__device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedItem &it, FewLds<DH> &lds) {
     constexpr int CW = DH / 16, KS = DH / 32;  // columns of v per lane, contraction steps of q . k
-    __shared__ float s_m[4][16], s_l[4][16], s_o[4][CW * 4][WAVE];
-    PagedItem it;
-    if (!paged_item<16>(p, it)) return;
     const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, j = lane % 16, g = lane / 16;
     const uint32_t row = it.row0 + min(j, it.nrows - 1), token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
     const uint32_t keep = paged_keep(p, it, token), keys = paged_keep(p, it, fastdiv(it.row0 + it.nrows - 1, p.group));
@@ -269,19 +321,19 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
     l += __shfl_xor(l, 32, WAVE);
 
     // the four waves' results, on one maximum
-    if (g == 0) s_m[wave][j] = m, s_l[wave][j] = l;
+    if (g == 0) lds.m[wave][j] = m, lds.l[wave][j] = l;
     __syncthreads();
-    float top = s_m[0][j];
+    float top = lds.m[0][j];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, s_m[w][j]);
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, lds.m[w][j]);
     const float ref = top == -INFINITY ? 0.f : top, f = __builtin_amdgcn_exp2f(m - ref);
     float total = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) total += s_l[w][j] * __builtin_amdgcn_exp2f(s_m[w][j] - ref);
+    for (int w = 0; w < 4; ++w) total += lds.l[w][j] * __builtin_amdgcn_exp2f(lds.m[w][j] - ref);
 #pragma unroll
     for (int t = 0; t < CW; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_o[wave][4 * t + i][lane] = o[t][i] * f;
+        for (int i = 0; i < 4; ++i) lds.o[wave][4 * t + i][lane] = o[t][i] * f;
     __syncthreads();
     // lane (j, g) of wave i: query j, columns CW (4 g + i) .. + CW - 1
     if (j >= it.nrows) return;
@@ -290,14 +342,14 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
     for (int t = 0; t < CW; ++t) {
         out[t] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) out[t] += s_o[w][4 * t + wave][lane];
+        for (int w = 0; w < 4; ++w) out[t] += lds.o[w][4 * t + wave][lane];
     }
     const uint32_t column = CW * (4 * g + wave);
     if (it.pieces > 1) {
-        float *dst = paged_partial(p, 16) + ((size_t)it.slot * 16 + j) * DH + column;
+        float *dst = paged_partial(p, ROWS) + ((size_t)it.slot * ROWS + j) * DH + column;
 #pragma unroll
         for (int t = 0; t < CW; t += 4) *reinterpret_cast<f32x4 *>(dst + t) = f32x4{out[t], out[t + 1], out[t + 2], out[t + 3]};
-        if (column == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * 16 + j) * 2) = f32x2{top, total};
+        if (column == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + j) * 2) = f32x2{top, total};
         return;
     }
     const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
@@ -328,15 +380,17 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int DH>
-__device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
-    constexpr int BN = 64;
-    constexpr int KP = DH + 8, VP = DH + 32;  // pitches of a row in LDS: reads of consecutive rows spread over the banks
+struct ManyLds {
+    static constexpr int BN = 64;                    // keys of a tile
+    static constexpr int KP = DH + 8, VP = DH + 32;  // pitches of a row: reads of consecutive rows spread over the banks
+    elem k[2][BN * KP], v[2][BN * VP];
+};
+
+template <int DH>
+__device__ __forceinline__ void paged_many(const AttnPagedParams &p, const PagedItem &it, ManyLds<DH> &lds) {
+    constexpr int BN = ManyLds<DH>::BN, KP = ManyLds<DH>::KP, VP = ManyLds<DH>::VP;
     constexpr int CPR = DH / 8, NCH = BN * CPR / 256, RS = 256 / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
     constexpr int DS = DH / 16, DB = DH / 32;
-    __shared__ __attribute__((aligned(16))) elem k_lds[2][BN * KP];
-    __shared__ __attribute__((aligned(16))) elem v_lds[2][BN * VP];
-    PagedItem it;
-    if (!paged_item<128>(p, it)) return;
     const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
     const uint32_t n32 = lane % 32, h = lane / 32, s16 = lane % 16, b16 = (lane / 16) % 2;
     const uint32_t wrow = wave * 32, at = min(wrow + n32, it.nrows - 1);
@@ -406,8 +460,8 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     auto commit = [&](int buf) {
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
-            st128(&k_lds[buf][(cr + RS * i) * KP + 8 * cc], kreg[i]);
-            st128(&v_lds[buf][(cr + RS * i) * VP + 8 * cc], vreg[i]);
+            st128(&lds.k[buf][(cr + RS * i) * KP + 8 * cc], kreg[i]);
+            st128(&lds.v[buf][(cr + RS * i) * VP + 8 * cc], vreg[i]);
         }
     };
     f32x16 o[DB];
@@ -435,7 +489,7 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
             look_up(t + 2);
         }
         if ((int32_t)(t * BN) < lim_last) {
-            const elem *kt = k_lds[buf], *vt = v_lds[buf];
+            const elem *kt = lds.k[buf], *vt = lds.v[buf];
             __builtin_amdgcn_s_setprio(1);
             // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
             f32x16 sacc[2];
@@ -571,6 +625,24 @@ __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
 #pragma unroll
         for (int i = 0; i < W; ++i) dst[i] = f2e(out[i] * inv);
     }
+}
+
+template <int DH>
+__device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
+    __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
+    PagedItem it;
+    if (paged_item<16>(p, it)) paged_few<DH, 16>(p, it, lds);
+}
+template <int DH>
+__device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
+    __shared__ __attribute__((aligned(16))) union {
+        FewLds<DH> few;
+        ManyLds<DH> many;
+    } lds;
+    PagedItem it;
+    if (!paged_item<128>(p, it)) return;
+    if (it.s.n * p.group.d <= FEW) paged_few<DH, 128>(p, it, lds.few);
+    else paged_many<DH>(p, it, lds.many);
 }
 
 #define ATTN_PAGED(DH)                                                                                                                                   \

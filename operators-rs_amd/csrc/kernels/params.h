@@ -290,7 +290,6 @@ struct AttnPagedParams {
     uint32_t nkvh, dh, causal;
     uint32_t slots;     // key ranges the work area holds, and the number that the tiles are split into together; 0: no splitting
     uint32_t narrow;  // both caches of one layout, and distances inside a page, a row of the table and from page to page of less than 32 bits
-    uint32_t min_steps;  // a range has at least this many steps of 32 keys
     float scale;
 };
 

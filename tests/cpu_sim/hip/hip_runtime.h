@@ -173,6 +173,7 @@ inline T cpusim_read_lane(int line, T v, uint32_t src) {
 }
 // (the last parameter of each: the line of the call, by which the scheduler checks that the lanes that meet are at the
 // same operation)
+#define __builtin_amdgcn_readlane(v, src) cpusim_read_lane(__LINE__, v, (uint32_t)(src))
 template <class T>
 inline T __shfl_xor(T v, int mask, int = 64, int line = __builtin_LINE()) {
     return cpusim_read_lane(line, v, cpusim::lane_id() ^ (uint32_t)mask);

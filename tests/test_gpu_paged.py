@@ -158,6 +158,24 @@ def attend(gpu, stream, b, mask, **kw):
     return decode(b.o.back(stream), b.kind)
 
 
+def _many_sequences(count, seed):
+    rng = np.random.default_rng(seed)
+    lens = [(1, int(l)) for l in rng.integers(1, 60, count)]
+    for i in rng.integers(0, count, 4):
+        lens[i] = (int(rng.integers(2, 30)), 400)
+    lens[count // 2] = (0, 20)
+    return lens
+
+
+@pytest.mark.parametrize("count", [63, 64, 65, 300, 600])
+@pytest.mark.parametrize("group", [2, 20])
+def test_attention_paged_many_sequences(gpu, stream, count, group):
+    """More sequences than lanes of a wave and than threads of a workgroup: each finds its work in the prefix sums."""
+    b = Batch(gpu, np.random.default_rng(16), "f16", group, 1, 64, 16, _many_sequences(count, count), pad=2)
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
 SHAPES = [  # nh, nkvh, dh, page, lens
     (4, 4, 64, 16, [(1, 1)]),
     (4, 1, 64, 16, [(1, 33), (1, 16), (1, 0), (1, 300)]),
