@@ -245,7 +245,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         const int e = m.dt == OPHIP_DT_BF16, h = dh == 128;
         op->dev->make_current();
         launch(op->rows[e][plan.many][h], Dim3{(unsigned)plan.grid}, Dim3{256}, 0, stream_of(qa), p);
-        if (plan.slots) launch(op->join[e][plan.many][h], Dim3{(unsigned)plan.slots, plan.many ? 4u : 1u}, Dim3{256}, 0, stream_of(qa), p);
+        if (plan.slots) launch(op->join[e][plan.many][h], Dim3{(unsigned)plan.slots}, Dim3{256}, 0, stream_of(qa), p);
         return;
     }
     op->dev->make_current();

@@ -55,14 +55,18 @@ __device__ __forceinline__ uint32_t paged_tiles(const AttnPagedParams &p, const 
     return rows <= FEW ? (rows ? 1 : 0) : (uint32_t)((rows + ROWS - 1) / ROWS);
 }
 __device__ __forceinline__ uint32_t paged_steps(const PagedSeq &s) { return (s.len + 31) / 32; }
-// Key ranges that a sequence's tiles are cut into, from the ranges that a step of 32 keys is worth
+// What a step of 32 keys costs a workgroup, roughly: twice as much where a tile's rows fill the matrix cores
+__device__ __forceinline__ float paged_weight(const AttnPagedParams &p, const PagedSeq &s) {
+    return (uint64_t)s.n * p.group.d <= FEW ? (float)paged_steps(s) : 2.f * (float)paged_steps(s);
+}
+// Key ranges that a sequence's tiles are cut into, from the ranges that a unit of weight is worth
 template <int ROWS>
 __device__ __forceinline__ uint32_t paged_pieces(const AttnPagedParams &p, const PagedSeq &s, float per_step) {
     const uint32_t least = (uint64_t)s.n * p.group.d <= FEW ? 4 : 8;  // steps in a range: one for each wave, four tiles of 64 keys
     const uint32_t most = paged_steps(s) / least;
-    return p.slots && most > 1 ? min(most, max(1u, (uint32_t)((float)paged_steps(s) * per_step + 0.5f))) : 1;
+    return p.slots && most > 1 ? min(most, max(1u, (uint32_t)(paged_weight(p, s) * per_step + 0.5f))) : 1;
 }
-// `work`: tiles times steps of all sequences.  Three quarters of the slots: a count rounded to two or more is at most four
+// `work`: tiles times weight of all sequences.  Three quarters of the slots: a count rounded to two or more is at most four
 // thirds of what it was.
 __device__ __forceinline__ float paged_per_step(const AttnPagedParams &p, float work) {
     return work > 0.f ? 0.74999f * (float)p.slots / (work * (float)p.nkvh) : 0.f;
@@ -80,7 +84,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         PagedSeq s{0, 0, 0};
         if (on) s = paged_seq(p.b, lane);
         const uint32_t tiles = paged_tiles<ROWS>(p, s);
-        const float work = p.slots ? wave_sum_dpp((float)tiles * (float)paged_steps(s)) : 0.f;
+        const float work = p.slots ? wave_sum_dpp((float)tiles * paged_weight(p, s)) : 0.f;
         const uint32_t pieces = paged_pieces<ROWS>(p, s, paged_per_step(p, work));
         const uint32_t items = tiles * p.nkvh * pieces, slots = pieces > 1 ? items : 0;
         uint32_t items0 = 0, slots0 = 0, all_slots = 0;
@@ -109,7 +113,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
             float work = 0.f;
             for (uint32_t i = tid; i < p.b.nseq; i += 256) {
                 const PagedSeq s = paged_seq(p.b, i);
-                work += (float)paged_tiles<ROWS>(p, s) * (float)paged_steps(s);
+                work += (float)paged_tiles<ROWS>(p, s) * paged_weight(p, s);
             }
             work = wave_sum_dpp(work);
             if (lane == 0) s_work[wave] = work;
@@ -590,12 +594,12 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 
 // ---- the ranges of a cut tile: o = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
 //
-// Workgroup (slot, y): the rows of the slot's tile are dealt out to the workgroups of its ranges, a wave to a row, its lanes
-// the columns.
+// The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
+// way at a time, and the ranges are folded in one pass with a running maximum.
 template <int DH, int ROWS>
 __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
-    constexpr int W = DH / WAVE;  // columns per lane
-    const uint32_t slot = blockIdx.x, wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
+    constexpr int TPR = DH / 4, RPP = 256 / TPR;  // threads per row, rows per pass
+    const uint32_t slot = blockIdx.x, col = 4 * (threadIdx.x % TPR);
     const PagedDesc d = paged_desc(p)[slot];
     // Slots behind the count hold no descriptor; nor do those of a batch whose sequences overlap, when it has more tiles than
     // the grid allows for: what lies there must not lead outside the workspace or o.
@@ -603,27 +607,47 @@ __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
     const uint64_t before = (uint64_t)d.piece * p.nkvh, behind = (uint64_t)(d.pieces - 1 - d.piece) * p.nkvh;
     if (before > slot || slot + behind >= p.slots) return;
     const uint32_t slot0 = slot - (uint32_t)before;
-    for (uint32_t r = (d.piece * gridDim.y + blockIdx.y) * 4 + wave; r < d.nrows; r += d.pieces * gridDim.y * 4) {
-        const float *st = paged_stats(p) + ((size_t)slot0 * ROWS + r) * 2, *po = paged_partial(p, ROWS) + ((size_t)slot0 * ROWS + r) * DH + W * lane;
-        const size_t step = (size_t)p.nkvh * ROWS;
-        float top = -INFINITY;
-        for (uint32_t c = lane; c < d.pieces; c += WAVE) top = fmaxf(top, st[2 * step * c]);
-        top = wave_max(top);
-        const float ref = top == -INFINITY ? 0.f : top;
-        float total = 0.f, out[W] = {};
-#pragma unroll 8
-        for (uint32_t c = 0; c < d.pieces; ++c) {
-            const float f = __builtin_amdgcn_exp2f(st[2 * step * c] - ref);
-            total += f * st[2 * step * c + 1];
+    const size_t step = (size_t)p.nkvh * ROWS;
+    for (uint32_t r = d.piece * RPP + threadIdx.x / TPR; r < d.nrows; r += d.pieces * RPP) {
+        const float *st = paged_stats(p) + ((size_t)slot0 * ROWS + r) * 2, *po = paged_partial(p, ROWS) + ((size_t)slot0 * ROWS + r) * DH + col;
+        float top = -INFINITY, total = 0.f;
+        f32x4 out = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t c0 = 0; c0 < d.pieces; c0 += 4) {
+            f32x2 ml[4];
+            f32x4 o[4];
 #pragma unroll
-            for (int i = 0; i < W; ++i) out[i] += f * po[step * DH * c + i];
+            for (uint32_t i = 0; i < 4; ++i) {
+                const uint32_t c = min(c0 + i, d.pieces - 1);
+                ml[i] = *reinterpret_cast<const f32x2 *>(st + 2 * step * c);
+                o[i] = *reinterpret_cast<const f32x4 *>(po + step * DH * c);
+            }
+            float now = top;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                if (c0 + i >= d.pieces) ml[i] = f32x2{-INFINITY, 0.f};
+                now = fmaxf(now, ml[i][0]);
+            }
+            const float ref = now == -INFINITY ? 0.f : now, old = __builtin_amdgcn_exp2f(top - ref);
+            total *= old;
+            out *= old;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) {
+                const float f = __builtin_amdgcn_exp2f(ml[i][0] - ref);
+                total += f * ml[i][1];
+                if (c0 + i < d.pieces) out += f * o[i];
+            }
+            top = now;
         }
         const float inv = total == 0.f ? 0.f : 1.0f / total;
         const uint32_t row = d.row0 + r, token = fastdiv(row, p.group), head = d.kvh * p.group.d + (row - token * p.group.d);
         if (d.start >= p.b.nt || token >= p.b.nt - d.start) return;
-        elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(d.start + token) * p.o_st) + W * lane;
+        union {
+            elem e[4];
+            u32x2 u;
+        } y;
 #pragma unroll
-        for (int i = 0; i < W; ++i) dst[i] = f2e(out[i] * inv);
+        for (int i = 0; i < 4; ++i) y.e[i] = f2e(out[i] * inv);
+        *reinterpret_cast<u32x2 *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(d.start + token) * p.o_st + 2 * col) = y.u;
     }
 }
 
