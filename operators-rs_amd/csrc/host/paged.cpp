@@ -287,11 +287,11 @@ int ophip_attention_paged_launch(const ophip_attention_paged *op, const ophip_at
 // ============================================================== kv_append_paged ===
 
 struct ophip_kv_append_paged : OpBase {
-    hipFunction_t vec[3], pairs[3];
+    hipFunction_t vec[3][2], pairs[3];  // vec: plain and non-temporal stores
     explicit ophip_kv_append_paged(ophip_device *d) : OpBase(d) {
         static const char *tag[3] = {"f16", "bf16", "f32"};
         for (int t = 0; t < 3; ++t) {
-            vec[t] = d->kernel("kv_append_paged", (std::string("kv_append_") + tag[t] + "_vec").c_str());
+            for (int nt = 0; nt < 2; ++nt) vec[t][nt] = d->kernel("kv_append_paged", (std::string("kv_append_") + tag[t] + (nt ? "_vec_nt" : "_vec")).c_str());
             pairs[t] = d->kernel("kv_append_paged", (std::string("kv_append_") + tag[t] + "_pairs").c_str());
         }
     }
@@ -358,7 +358,10 @@ void kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_appe
     const bool vec = dh * ophip_dtype_nbytes(m.dt) % 16 == 0 && vector_rows(a.k_layout, a.k_base) && vector_rows(a.v_layout, a.v_base) &&
                      vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base);
     op->dev->make_current();
-    launch((vec ? op->vec : op->pairs)[type_index(m.dt)], Dim3{(unsigned)nt}, Dim3{256}, p.rotate ? dh / 2 * 8 : 0, stream_of(qa), p);
+    // (more than the L2 caches hold together, 8 x 4 MiB: whoever reads it next does not find it there)
+    const bool stream_out = 2 * nt * nkvh * dh * ophip_dtype_nbytes(m.dt) > (size_t)32 << 20;
+    const int t = type_index(m.dt);
+    launch(vec ? op->vec[t][stream_out] : op->pairs[t], Dim3{(unsigned)nt}, Dim3{256}, p.rotate ? dh / 2 * 8 : 0, stream_of(qa), p);
 }
 
 }  // namespace
@@ -393,12 +396,13 @@ int ophip_kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv
 // ================================================================= qk_norm_rope ===
 
 struct ophip_qk_norm_rope : OpBase {
-    hipFunction_t vec[3][4], pairs[3];  // vec: rows of 8, 16, 32, 64 lanes
+    hipFunction_t vec[3][4][2], pairs[3];  // vec: rows of 8, 16, 32, 64 lanes; plain and non-temporal stores
     explicit ophip_qk_norm_rope(ophip_device *d) : OpBase(d) {
         static const char *tag[3] = {"f16", "bf16", "f32"}, *lanes[4] = {"_l8", "_l16", "_l32", "_l64"};
         for (int t = 0; t < 3; ++t) {
             const std::string name = std::string("qk_norm_rope_") + tag[t];
-            for (int l = 0; l < 4; ++l) vec[t][l] = d->kernel("qk_norm_rope", (name + lanes[l]).c_str());
+            for (int l = 0; l < 4; ++l)
+                for (int nt = 0; nt < 2; ++nt) vec[t][l][nt] = d->kernel("qk_norm_rope", (name + lanes[l] + (nt ? "_nt" : "")).c_str());
             pairs[t] = d->kernel("qk_norm_rope", (name + "_pairs").c_str());
         }
     }
@@ -476,14 +480,16 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     vec = vec && vectors <= 64;
     const int li = vectors <= 8 ? 0 : vectors <= 16 ? 1 : vectors <= 32 ? 2 : 3;
     // Few tokens: a token's heads over several workgroups, down to one row for each group of lanes.  Many: several tokens to
-    // a workgroup, so that each of its 256 threads has one pair's sine and cosine to evaluate.
-    const size_t rows = vec ? 32u >> li : 4, tokens = vec && nt >= 4096 ? std::max<size_t>(1, 512 / dh) : 1;
+    // a workgroup, two pairs of sine and cosine for each of its 256 threads.  Stores are non-temporal where
+    // the result is larger than the L2 caches together (8 x 4 MiB): whoever reads it next does not find it there.
+    const size_t rows = vec ? 32u >> li : 4, tokens = vec && nt >= 4096 ? std::max<size_t>(1, 1024 / dh) : 1;
+    const bool stream_out = nt * heads * dh * unit > (size_t)32 << 20;
     const size_t by = tokens > 1 ? 1 : std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt)), per = (heads + by - 1) / by;
     p.heads_per_block = make_fastdiv((uint32_t)per);
     p.tokens_per_block = (uint32_t)tokens;
     op->dev->make_current();
     const int t = type_index(m.dt);
-    launch(vec ? op->vec[t][li] : op->pairs[t], Dim3{(unsigned)((nt + tokens - 1) / tokens), (unsigned)((heads + per - 1) / per)}, Dim3{256},
+    launch(vec ? op->vec[t][li][stream_out] : op->pairs[t], Dim3{(unsigned)((nt + tokens - 1) / tokens), (unsigned)((heads + per - 1) / per)}, Dim3{256},
            p.rotate ? tokens * (dh / 2) * 8 : 0, stream_of(qa), p);
 }
 

@@ -3,10 +3,11 @@
 // A workgroup serves some consecutive tokens, or one slice of one token's nh + nkh heads when there are few.  A row (one
 // head) is 16 bytes in each of L consecutive lanes, so its sum of squares is a sum over L lanes and everything else stays
 // in the lane: each byte is read once and written once, and what bounds the kernel is memory.  The tokens' sines and
-// cosines are evaluated once into LDS, a pair of a token per thread, while the first rows travel: 256 / (dh / 2) tokens
-// give every thread one (an evaluation is some fifty f64 instructions; a token per workgroup leaves three
-// quarters of the threads of dh 128 waiting for it: 65 us against 45 for 8191 tokens of 40 heads), and four rows per
-// thread are on their way at a time.
+// cosines are evaluated once into LDS, a pair of a token per thread, while the first rows travel (an evaluation is some fifty
+// f64 instructions behind the load of a position), and four rows per thread are on their way at a time.  8191 tokens of 40
+// heads of 128 (168 MB moved), on one machine: 73 us with a token per workgroup, 59 with two, 49 with four, 45.5 with eight,
+// 48 with sixteen; with non-temporal stores 41 (4.1 TB/s; a plain copy of 4 GiB 4.9), with the next rows requested before
+// the present ones are worked on 40.4: not worth the registers.
 #include "paged.h"
 
 extern __shared__ float2 qk_sc[];  // [token][dh / 2] of (sin, cos)
@@ -21,7 +22,8 @@ __device__ __forceinline__ void qk_fill_table(const QkNormRopeParams &p, uint32_
 }
 
 // Rows of whole 16-byte vectors, aligned; L = the power of two of lanes that holds one (lanes past dh idle)
-template <typename T, int L>
+// (NT: with the non-temporal hint on the stores)
+template <typename T, int L, bool NT>
 __device__ __forceinline__ void qk_norm_rope_vec(const QkNormRopeParams &p) {
     constexpr int E = 16 / sizeof(T), G = WG_THREADS / L, U = 4;
     const uint32_t token0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.nt - token0), lane = threadIdx.x % L;
@@ -86,7 +88,9 @@ __device__ __forceinline__ void qk_norm_rope_vec(const QkNormRopeParams &p) {
             }
 #pragma unroll
             for (int i = 0; i < E; ++i) x[u].e[i] = (T)f[i];
-            st128(reinterpret_cast<char *>(p.y[which[u]]) + (int64_t)(token0 + tok[u]) * p.y_st[which[u]] + (int64_t)head[u] * p.y_sh[which[u]] + 16 * lane, x[u].u);
+            char *dst = reinterpret_cast<char *>(p.y[which[u]]) + (int64_t)(token0 + tok[u]) * p.y_st[which[u]] + (int64_t)head[u] * p.y_sh[which[u]] + 16 * lane;
+            if constexpr (NT) st128_nt(dst, x[u].u);
+            else st128(dst, x[u].u);
         }
     }
 }
@@ -119,11 +123,14 @@ __device__ __forceinline__ void qk_norm_rope_pairs(const QkNormRopeParams &p) {
     }
 }
 
-#define QK_NORM_ROPE(name, T)                                                                                                        \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l8(QkNormRopeParams p) { qk_norm_rope_vec<T, 8>(p); }    \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l16(QkNormRopeParams p) { qk_norm_rope_vec<T, 16>(p); }  \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l32(QkNormRopeParams p) { qk_norm_rope_vec<T, 32>(p); }  \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l64(QkNormRopeParams p) { qk_norm_rope_vec<T, 64>(p); }  \
+#define QK_NORM_ROPE_L(name, T, L)                                                                                                                \
+    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L(QkNormRopeParams p) { qk_norm_rope_vec<T, L, false>(p); }        \
+    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L##_nt(QkNormRopeParams p) { qk_norm_rope_vec<T, L, true>(p); }
+#define QK_NORM_ROPE(name, T)                                                                                                                     \
+    QK_NORM_ROPE_L(name, T, 8)                                                                                                                    \
+    QK_NORM_ROPE_L(name, T, 16)                                                                                                                   \
+    QK_NORM_ROPE_L(name, T, 32)                                                                                                                   \
+    QK_NORM_ROPE_L(name, T, 64)                                                                                                                   \
     extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_pairs(QkNormRopeParams p) { qk_norm_rope_pairs<T>(p); }
 QK_NORM_ROPE(f16, f16)
 QK_NORM_ROPE(bf16, bf16)

@@ -450,6 +450,11 @@ def test_kv_append_paged(gpu, stream, shape, theta, kind):
     check_append(gpu, stream, append_case(gpu, np.random.default_rng(20), kind, *shape, pad=2), theta)
 
 
+def test_kv_append_paged_more_than_the_caches_hold(gpu, stream):
+    """48 MiB of rows: non-temporal stores."""
+    check_append(gpu, stream, append_case(gpu, np.random.default_rng(26), "bf16", 32, 128, 64, [(1000, 1003), (2000, 2000)], 5), 10000.0)
+
+
 @pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap"])
 def test_kv_append_paged_views(gpu, stream, form):
     b = append_case(gpu, np.random.default_rng(21), "bf16", 2, 64, 16, [(3, 20), (1, 40)], 1, token_major=form == "token_major",
@@ -582,6 +587,12 @@ def test_qk_norm_rope_small_and_large_rows(gpu, stream, scale):
 
 def test_qk_norm_rope_many_tokens(gpu, stream):
     check_norm(gpu, stream, np.random.default_rng(33), 1500, 4, 1, 64, "bf16", "f32", 10000.0)
+
+
+@pytest.mark.parametrize("nt,nh,nkh,dh", [(4099, 2, 1, 64), (4096, 0, 1, 512), (4097, 3, 0, 8), (4100, 1, 2, 96), (4101, 32, 8, 128)])
+def test_qk_norm_rope_several_tokens_per_workgroup(gpu, stream, nt, nh, nkh, dh):
+    """From 4096 tokens on a workgroup takes several, the last one fewer; the largest result goes out in non-temporal stores."""
+    check_norm(gpu, stream, np.random.default_rng(34), nt, nh, nkh, dh, "f16", "f16", 10000.0)
 
 
 def test_qk_norm_rope_refusals(gpu, stream):
