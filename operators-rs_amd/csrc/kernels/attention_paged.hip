@@ -498,14 +498,21 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
             f32x16 sacc[2];
 #pragma unroll
-            for (int b = 0; b < 2; ++b) {
+            for (int b = 0; b < 2; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sacc[b][e] = 0.f;
+            {
+                constexpr int N = 2 * DS, AHEAD = 8;
+                PackE a[N];
+                auto load = [&](int i) { a[i].u = ld128(kt + (32 * (i % 2) + n32) * KP + 16 * (i / 2) + 8 * h); };
 #pragma unroll
-                for (int d = 0; d < DS; ++d) {
-                    PackE a;
-                    a.u = ld128(kt + (32 * b + n32) * KP + 16 * d + 8 * h);
-                    sacc[b] = mfma_32x32x16(a.h, qf[d].h, sacc[b]);
+                for (int i = 0; i < AHEAD; ++i) load(i);
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    sacc[i % 2] = mfma_32x32x16(a[i].h, qf[i / 2].h, sacc[i % 2]);
+                    if (i + AHEAD < N) load(i + AHEAD);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             }
             __builtin_amdgcn_s_setprio(0);
@@ -533,32 +540,41 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
                 m = now;
             }
             const float shift = PA_BIAS - (m == -INFINITY ? 0.f : m);  // (a row that has kept nothing so far: every term is 0)
-            float sum = 0.f;
             PackE pb[4];  // MFMA n: the tile's keys 16 n .. + 15, slots 8 h .. 8 h + 7 keys 16 n + 4 h + {0..3}, 16 n + 8 + 4 h + {0..3}
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift));
-                    sum += x;
-                    pb[2 * b + e / 8].e[e % 8] = f2e(x);
-                }
-            l += sum;
+            auto power = [&](int b, int e) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift));
+                l += x;
+                pb[2 * b + e / 8].e[e % 8] = f2e(x);
+            };
             typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
+            {
+                constexpr int N = 4 * DB, AHEAD = 4, EACH = 32 / N;  // powers of the second half with each of the first half's products
+                union Frag {
+                    s16x4 half[2];
+                    elem8 hv;
+                } a[N];
+                auto load = [&](int i) {
+                    const int n = i / DB, d = i % DB;
                     const elem *src = vt + (16 * n + 4 * h + s16 / 4) * VP + 32 * d + 16 * b16 + 4 * (s16 % 4);
-                    union {
-                        s16x4 half[2];
-                        elem8 hv;
-                    } a;
-                    a.half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)src);
-                    a.half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(src + 8 * VP));
-                    o[d] = mfma_32x32x16(a.hv, pb[n].h, o[d]);
+                    a[i].half[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)src);
+                    a[i].half[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(src + 8 * VP));
+                };
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) load(i);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) power(0, e);
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    o[i % DB] = mfma_32x32x16(a[i].hv, pb[i / DB].h, o[i % DB]);
+                    if (i + AHEAD < N) load(i + AHEAD);
+                    if (i < N / 2)
+#pragma unroll
+                        for (int e = EACH * i; e < EACH * (i + 1); ++e) power(1, e);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+            }
         }
         __builtin_amdgcn_s_setprio(0);
         if (more) commit(buf ^ 1);
