@@ -123,21 +123,24 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 
 struct ophip_attention_paged : OpBase {
     hipFunction_t any[3];
-    hipFunction_t rows[2][2][2], join[2][2][2];  // [f16 / bf16][tiles of 16 / 128 rows][dh 64 / 128]
-    int slots[2] = {0, 0};  // OPHIP_ATTN_PAGED_SLOTS=<few>,<many>: key ranges to cut a launch into (sweeps); read once, here
+    hipFunction_t rows[2][3][2], join[2][3][2];  // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64 / 128]
+    // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2
+    // one size of tile
+    int slots = 0, tile = -1;
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
         any[0] = d->kernel("attention_paged_any", "attn_paged_any_f16");
         any[1] = d->kernel("attention_paged_any", "attn_paged_any_bf16");
         any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
         for (int e = 0; e < 2; ++e)
-            for (int r = 0; r < 2; ++r)
+            for (int r = 0; r < 3; ++r)
                 for (int h = 0; h < 2; ++h) {
                     const char *mod = e ? "attention_paged_bf16" : "attention_paged";
-                    const std::string tail = std::string(r ? "many" : "few") + (h ? "_d128" : "_d64") + (e ? "_bf16" : "");
+                    const std::string tail = std::string(r == 0 ? "few" : r == 1 ? "many" : "wide") + (h ? "_d128" : "_d64") + (e ? "_bf16" : "");
                     rows[e][r][h] = d->kernel(mod, ("attn_paged_" + tail).c_str());
                     join[e][r][h] = d->kernel(mod, ("attn_paged_join_" + tail).c_str());
                 }
-        if (const char *e = std::getenv("OPHIP_ATTN_PAGED_SLOTS")) std::sscanf(e, "%d,%d", &slots[0], &slots[1]);
+        if (const char *e = std::getenv("OPHIP_ATTN_PAGED_SLOTS")) slots = std::atoi(e);
+        if (const char *e = std::getenv("OPHIP_ATTN_PAGED_TILE")) tile = std::atoi(e);
     }
 };
 
@@ -166,7 +169,7 @@ AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
 // How the matrix kernels take a call (attention_paged.hip), from its sizes alone.
 struct AttnPagedPlan {
     bool matrix;                    // they serve these types and sizes
-    int many;                       // tiles of 128 rows, or of 16
+    int tile;                       // tiles of 16, 128 or 256 rows: 0, 1, 2
     size_t grid, slots;  // workgroups; key ranges the workspace holds (0: no tile can be cut)
     size_t workspace;
 };
@@ -177,19 +180,23 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || (m.dh != 64 && m.dh != 128) || m.nh % m.nkvh) return a;
     if (m.nh > MAX_INDEX / m.nt || m.page > MAX_INDEX / m.cols) return a;
     a.matrix = true;
-    // up to 16 rows per sequence and kv head on average: nearly all of it is decode steps
+    // Rows per sequence and kv head, on average.  Up to 16: nearly all of it is decode steps.  From 1024 on: 256-row tiles, which
+    // load once for twice the rows, and whose last one may stay as empty as it likes (8192 tokens, 32 heads over 8: 558 against
+    // 585 us, 511 tokens over 32511 keys 299 against 318; prompts of 104 .. 546 tokens 36.8 against 32.6).
     const size_t group = m.nh / m.nkvh, rows = m.nt * group;
-    a.many = rows > 16 * m.nseq;
-    const size_t tile = a.many ? 128 : 16;
+    a.tile = rows <= 16 * m.nseq ? 0 : rows < 1024 * m.nseq ? 1 : 2;
+    if (op && op->tile >= 0 && op->tile <= 2) a.tile = op->tile;
+    const size_t tile = a.tile == 0 ? 16 : a.tile == 1 ? 128 : 256;
     // the most tiles there can be, whatever the lengths: each sequence that has a token may have one that is not full
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
     const size_t steps = (m.cols * m.page + 31) / 32;
     const size_t most = std::max<size_t>(1, steps / 4);  // (a key range has four steps of 32 keys at least)
-    // Key ranges for all tiles together: as many as workgroups of 128 rows run at a time (two per CU; 511 tokens over 32511
-    // keys, 32 heads over 8: 420 us with half as many, 321, 338 with twice as many), and twice that for 16 rows, where a range costs
-    // little and the rates of memory even out (50 decode steps over 165008 keys: 134 us with 512, 122 with 1024, 124 with 1536).
+    // Key ranges for all tiles together: as many as workgroups of 128 or 256 rows run at a time (two or one per CU; 511 tokens over
+    // 32511 keys, 32 heads over 8, on tiles of 128: 420 us with half as many, 321, 338 with twice as many), and four per CU
+    // for 16 rows, where a range costs little and the rates of memory even out (50 decode steps over 165008 keys: 134 us
+    // with 512, 122 with 1024, 124 with 1536).
     const size_t cus = (size_t)(op ? op->dev->props.multiProcessorCount : 256);
-    const size_t want = op && op->slots[a.many] > 0 ? (size_t)op->slots[a.many] : (a.many ? 2 : 4) * cus;
+    const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 ? 2 : 1) * cus;
     a.grid = units;
     if (most > 1) {
         a.slots = std::min((4 * want + 2) / 3, units * most);
@@ -244,8 +251,8 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
                    p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;
         const int e = m.dt == OPHIP_DT_BF16, h = dh == 128;
         op->dev->make_current();
-        launch(op->rows[e][plan.many][h], Dim3{(unsigned)plan.grid}, Dim3{256}, 0, stream_of(qa), p);
-        if (plan.slots) launch(op->join[e][plan.many][h], Dim3{(unsigned)plan.slots}, Dim3{256}, 0, stream_of(qa), p);
+        launch(op->rows[e][plan.tile][h], Dim3{(unsigned)plan.grid}, Dim3{plan.tile == 2 ? 512u : 256u}, 0, stream_of(qa), p);
+        if (plan.slots) launch(op->join[e][plan.tile][h], Dim3{(unsigned)plan.slots}, Dim3{256}, 0, stream_of(qa), p);
         return;
     }
     op->dev->make_current();

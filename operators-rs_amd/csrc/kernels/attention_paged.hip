@@ -73,7 +73,7 @@ __device__ __forceinline__ float paged_per_step(const AttnPagedParams &p, float 
 }
 
 // What workgroup blockIdx.x does; false: nothing.  Every thread calls it and gets the same.
-template <int ROWS>
+template <int ROWS, int WAVES>
 __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &it) {
     const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE, w = blockIdx.x;
     uint32_t local, first_slot;
@@ -105,13 +105,14 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         local = w - __builtin_amdgcn_readlane(items0, at);
         first_slot = __builtin_amdgcn_readlane(slots0, at);
     } else {
-        __shared__ float s_work[4];
-        __shared__ uint32_t s_scan[2][4], s_found[4];
+        constexpr uint32_t THREADS = WAVES * WAVE;
+        __shared__ float s_work[WAVES];
+        __shared__ uint32_t s_scan[2][WAVES], s_found[4];
         float per_step = 0.f;
         if (tid == 0) s_found[0] = 0xffffffffu;
         if (p.slots) {
             float work = 0.f;
-            for (uint32_t i = tid; i < p.b.nseq; i += 256) {
+            for (uint32_t i = tid; i < p.b.nseq; i += THREADS) {
                 const PagedSeq s = paged_seq(p.b, i);
                 work += (float)paged_tiles<ROWS>(p, s) * paged_weight(p, s);
             }
@@ -119,9 +120,14 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
             if (lane == 0) s_work[wave] = work;
         }
         __syncthreads();
-        if (p.slots) per_step = paged_per_step(p, s_work[0] + s_work[1] + s_work[2] + s_work[3]);
+        if (p.slots) {
+            float work = 0.f;
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) work += s_work[v];
+            per_step = paged_per_step(p, work);
+        }
         uint32_t items0 = 0, slots0 = 0;
-        for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += 256) {
+        for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += THREADS) {
             uint32_t items = 0, slots = 0, pieces = 1;
             if (i0 + tid < p.b.nseq) {
                 const PagedSeq s = paged_seq(p.b, i0 + tid);
@@ -139,7 +145,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
             __syncthreads();
             uint32_t ta = 0, tb = 0;
 #pragma unroll
-            for (uint32_t v = 0; v < 4; ++v) {
+            for (uint32_t v = 0; v < WAVES; ++v) {
                 if (v < wave) a += s_scan[0][v], b += s_scan[1][v];
                 ta += s_scan[0][v], tb += s_scan[1][v];
             }
@@ -390,10 +396,10 @@ struct ManyLds {
     elem k[2][BN * KP], v[2][BN * VP];
 };
 
-template <int DH>
+template <int DH, int W>
 __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const PagedItem &it, ManyLds<DH> &lds) {
     constexpr int BN = ManyLds<DH>::BN, KP = ManyLds<DH>::KP, VP = ManyLds<DH>::VP;
-    constexpr int CPR = DH / 8, NCH = BN * CPR / 256, RS = 256 / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
+    constexpr int CPR = DH / 8, ROWS = 32 * W, NCH = BN * CPR / (W * WAVE), RS = W * WAVE / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
     constexpr int DS = DH / 16, DB = DH / 32;
     const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
     const uint32_t n32 = lane % 32, h = lane / 32, s16 = lane % 16, b16 = (lane / 16) % 2;
@@ -584,12 +590,12 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
     if (wrow + n32 >= it.nrows) return;
     // o[d][4 q + r]: column 32 d + 8 q + 4 h + r of the lane's query
     if (it.pieces > 1) {
-        float *dst = paged_partial(p, 128) + ((size_t)it.slot * 128 + at) * DH + 4 * h;
+        float *dst = paged_partial(p, ROWS) + ((size_t)it.slot * ROWS + at) * DH + 4 * h;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
             for (int q = 0; q < 4; ++q) *reinterpret_cast<f32x4 *>(dst + 32 * d + 8 * q) = f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
-        if (h == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * 128 + at) * 2) = f32x2{m, total};
+        if (h == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + at) * 2) = f32x2{m, total};
         return;
     }
     const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
@@ -671,24 +677,28 @@ template <int DH>
 __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
     __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
     PagedItem it;
-    if (paged_item<16>(p, it)) paged_few<DH, 16>(p, it, lds);
+    if (paged_item<16, 4>(p, it)) paged_few<DH, 16>(p, it, lds);
 }
-template <int DH>
+// W waves of 32 rows: 4, two workgroups to a CU, or 8, one
+template <int DH, int W>
 __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     __shared__ __attribute__((aligned(16))) union {
         FewLds<DH> few;
         ManyLds<DH> many;
     } lds;
     PagedItem it;
-    if (!paged_item<128>(p, it)) return;
-    if (it.s.n * p.group.d <= FEW) paged_few<DH, 128>(p, it, lds.few);
-    else paged_many<DH>(p, it, lds.many);
+    if (!paged_item<32 * W, W>(p, it)) return;
+    if (it.s.n * p.group.d <= FEW) {
+        if (threadIdx.x < 4 * WAVE) paged_few<DH, 32 * W>(p, it, lds.few);  // (waves that have ended are not waited for)
+    } else paged_many<DH, W>(p, it, lds.many);
 }
 
 #define ATTN_PAGED(DH)                                                                                                                                   \
     extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_few_d##DH)(AttnPagedParams p) { attn_paged_few<DH>(p); }                  \
-    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH>(p); }                \
+    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 4>(p); }             \
+    extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 8>(p); }             \
     extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 16>(p); }           \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }         \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 256>(p); }
 ATTN_PAGED(64)
 ATTN_PAGED(128)

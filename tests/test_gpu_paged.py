@@ -225,6 +225,29 @@ def test_attention_paged_keys_split_over_workgroups(gpu, stream, lens, kind):
     assert np.array_equal(one, two)  # the same bits
 
 
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+@pytest.mark.parametrize("mask", [1, 0])
+@pytest.mark.parametrize("lens", [[(1, 700), (3, 9), (0, 5)], [(300, 330)], [(17, 400), (1, 1500), (40, 40)], [(1100, 1100)], [(5, 2)] + [(1, 30)] * 66 + [(30, 600)]],
+                         ids=["decode", "prompt", "mixed", "long", "many"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_every_size_of_tile(gpu, stream, monkeypatch, tile, lens, mask, dh):
+    """Each kernel on every kind of batch, also those that another would be chosen for."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(17), "f16", 2, 1, dh, 24, lens, pad=1)
+    want, tol = b.expected(mask)
+    check(attend(gpu, stream, b, mask), want, tol)
+
+
+@pytest.mark.parametrize("tile", ["1", "2"])
+@pytest.mark.parametrize("slots", ["3", "40"])
+def test_attention_paged_few_and_many_key_ranges(gpu, stream, monkeypatch, tile, slots):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_SLOTS", slots)
+    b = Batch(gpu, np.random.default_rng(18), "bf16", 4, 2, 64, 16, [(20, 2000), (1, 3000), (70, 900)])
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
 @pytest.mark.parametrize("shape", [(4, 2, 64, 16, [(1, 90), (1, 40)]), (4, 2, 128, 16, [(50, 90), (1, 40)])], ids=["few", "many"])
 @pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap", "fused_qkv", "o_over_q", "strided_batch"])
 def test_attention_paged_views(gpu, stream, form, shape):
