@@ -287,12 +287,15 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
             m = now;
         }
         const float ref = m == -INFINITY ? 0.f : m;
-        PackE pr;
+        // A probability goes in as two elements, its rounding and what that left out: the matrix cores have the time, and the
+        // result then is as exact as with f32 probabilities.
+        PackE pr, rest;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float e = __builtin_amdgcn_exp2f(x[i] - ref + PA_BIAS);
             l += e;
             pr.e[i] = f2e(e);
+            rest.e[i] = f2e(e - e2f(pr.e[i]));
         }
 #pragma unroll
         for (int c = 0; c < CW; ++c) {
@@ -303,6 +306,7 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
                 a.u[d] = (c & 1) ? ((lo >> 16) | (hi & 0xffff0000u)) : ((lo & 0xffffu) | (hi << 16));
             }
             o[c] = mfma_16x16x32(a.h, pr.h, o[c]);
+            o[c] = mfma_16x16x32(a.h, rest.h, o[c]);
         }
     };
     if (first < last) {
