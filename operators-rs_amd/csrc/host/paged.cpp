@@ -403,13 +403,13 @@ int ophip_kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv
 // ================================================================= qk_norm_rope ===
 
 struct ophip_qk_norm_rope : OpBase {
-    hipFunction_t vec[3][4][2], pairs[3];  // vec: rows of 8, 16, 32, 64 lanes; plain and non-temporal stores
+    hipFunction_t vec[3][4][3], pairs[3];  // vec: rows of 8, 16, 32, 64 lanes; one row per thread, several, several with non-temporal stores
     explicit ophip_qk_norm_rope(ophip_device *d) : OpBase(d) {
-        static const char *tag[3] = {"f16", "bf16", "f32"}, *lanes[4] = {"_l8", "_l16", "_l32", "_l64"};
+        static const char *tag[3] = {"f16", "bf16", "f32"}, *lanes[4] = {"_l8", "_l16", "_l32", "_l64"}, *form[3] = {"", "_multi", "_multi_nt"};
         for (int t = 0; t < 3; ++t) {
             const std::string name = std::string("qk_norm_rope_") + tag[t];
             for (int l = 0; l < 4; ++l)
-                for (int nt = 0; nt < 2; ++nt) vec[t][l][nt] = d->kernel("qk_norm_rope", (name + lanes[l] + (nt ? "_nt" : "")).c_str());
+                for (int f = 0; f < 3; ++f) vec[t][l][f] = d->kernel("qk_norm_rope", (name + lanes[l] + form[f]).c_str());
             pairs[t] = d->kernel("qk_norm_rope", (name + "_pairs").c_str());
         }
     }
@@ -490,13 +490,12 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     // a workgroup, two pairs of sine and cosine for each of its 256 threads.  Stores are non-temporal where
     // the result is larger than the L2 caches together (8 x 4 MiB): whoever reads it next does not find it there.
     const size_t rows = vec ? 32u >> li : 4, tokens = vec && nt >= 4096 ? std::max<size_t>(1, 1024 / dh) : 1;
-    const bool stream_out = nt * heads * dh * unit > (size_t)32 << 20;
     const size_t by = tokens > 1 ? 1 : std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt)), per = (heads + by - 1) / by;
     p.heads_per_block = make_fastdiv((uint32_t)per);
     p.tokens_per_block = (uint32_t)tokens;
     op->dev->make_current();
-    const int t = type_index(m.dt);
-    launch(vec ? op->vec[t][li][stream_out] : op->pairs[t], Dim3{(unsigned)((nt + tokens - 1) / tokens), (unsigned)((heads + per - 1) / per)}, Dim3{256},
+    const int t = type_index(m.dt), form = tokens * per <= rows ? 0 : nt * heads * dh * unit <= (size_t)32 << 20 ? 1 : 2;
+    launch(vec ? op->vec[t][li][form] : op->pairs[t], Dim3{(unsigned)((nt + tokens - 1) / tokens), (unsigned)((heads + per - 1) / per)}, Dim3{256},
            p.rotate ? tokens * (dh / 2) * 8 : 0, stream_of(qa), p);
 }
 

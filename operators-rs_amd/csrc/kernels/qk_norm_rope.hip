@@ -4,7 +4,8 @@
 // head) is 16 bytes in each of L consecutive lanes, so its sum of squares is a sum over L lanes and everything else stays
 // in the lane: each byte is read once and written once, and what bounds the kernel is memory.  The tokens' sines and
 // cosines are evaluated once into LDS, a pair of a token per thread, while the first rows travel (an evaluation is some fifty
-// f64 instructions behind the load of a position), and four rows per thread are on their way at a time.  8191 tokens of 40
+// f64 instructions behind the load of a position), and four rows per thread are on their way at a time (one where a few tokens
+// leave a thread no more).  8191 tokens of 40
 // heads of 128 (168 MB moved), on one machine: 73 us with a token per workgroup, 59 with two, 49 with four, 45.5 with eight,
 // 48 with sixteen; with non-temporal stores 41 (4.1 TB/s; a plain copy of 4 GiB 4.9), with the next rows requested before
 // the present ones are worked on 40.4: not worth the registers.
@@ -22,10 +23,10 @@ __device__ __forceinline__ void qk_fill_table(const QkNormRopeParams &p, uint32_
 }
 
 // Rows of whole 16-byte vectors, aligned; L = the power of two of lanes that holds one (lanes past dh idle)
-// (NT: with the non-temporal hint on the stores)
-template <typename T, int L, bool NT>
+// U: rows of a thread on their way at a time; NT: with the non-temporal hint on the stores
+template <typename T, int L, int U, bool NT>
 __device__ __forceinline__ void qk_norm_rope_vec(const QkNormRopeParams &p) {
-    constexpr int E = 16 / sizeof(T), G = WG_THREADS / L, U = 4;
+    constexpr int E = 16 / sizeof(T), G = WG_THREADS / L;
     const uint32_t token0 = blockIdx.x * p.tokens_per_block, tokens = min(p.tokens_per_block, p.nt - token0), lane = threadIdx.x % L;
     const uint32_t heads = p.heads_per_block.d, h0 = blockIdx.y * heads, h1 = p.nh[0] + p.nh[1], rows = tokens * heads;
     const bool live = lane * E < p.dh;
@@ -123,9 +124,10 @@ __device__ __forceinline__ void qk_norm_rope_pairs(const QkNormRopeParams &p) {
     }
 }
 
-#define QK_NORM_ROPE_L(name, T, L)                                                                                                                \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L(QkNormRopeParams p) { qk_norm_rope_vec<T, L, false>(p); }        \
-    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L##_nt(QkNormRopeParams p) { qk_norm_rope_vec<T, L, true>(p); }
+#define QK_NORM_ROPE_L(name, T, L)                                                                                                                       \
+    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L(QkNormRopeParams p) { qk_norm_rope_vec<T, L, 1, false>(p); }            \
+    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L##_multi(QkNormRopeParams p) { qk_norm_rope_vec<T, L, 4, false>(p); }    \
+    extern "C" __global__ void __launch_bounds__(256) qk_norm_rope_##name##_l##L##_multi_nt(QkNormRopeParams p) { qk_norm_rope_vec<T, L, 4, true>(p); }
 #define QK_NORM_ROPE(name, T)                                                                                                                     \
     QK_NORM_ROPE_L(name, T, 8)                                                                                                                    \
     QK_NORM_ROPE_L(name, T, 16)                                                                                                                   \
