@@ -24,11 +24,14 @@ void expect_element_type(uint64_t dt) {
 }
 int type_index(uint64_t dt) { return dt == OPHIP_DT_F16 ? 0 : dt == OPHIP_DT_BF16 ? 1 : 2; }
 
-// every stride known and a whole number of elements
-void expect_strides(const ophip_tensor_layout &l, const char *name) {
+// every size and stride known, strides and address whole elements
+void expect_static(const ophip_tensor_layout &l, const void *base, const char *name) {
     const ptrdiff_t unit = (ptrdiff_t)ophip_dtype_nbytes(l.dt);
-    for (uint64_t i = 0; i < l.ndim; ++i)
+    for (uint64_t i = 0; i < l.ndim; ++i) {
+        (void)static_of(l.shape[i]);
         if (static_of(l.strides[i]) % unit != 0) throw strides_not_support(std::string("misaligned strides of ") + name);
+    }
+    if (reinterpret_cast<uintptr_t>(base) % (size_t)unit != 0) throw args_not_support(std::string("misaligned base of ") + name);
 }
 // elements adjacent, everything else on 16-byte boundaries
 bool vector_rows(const ophip_tensor_layout &l, const void *base) {
@@ -44,7 +47,7 @@ bool apart(const ophip_tensor_layout &a, const void *a_base, const ophip_tensor_
         const char *lo = static_cast<const char *>(base), *hi = lo + ophip_dtype_nbytes(l.dt);
         for (uint64_t i = 0; i < l.ndim; ++i) {
             if (l.shape[i] == 0) return std::pair<const char *, const char *>(nullptr, nullptr);
-            const ptrdiff_t reach = (ptrdiff_t)(l.shape[i] - 1) * l.strides[i];
+            const ptrdiff_t reach = (ptrdiff_t)((l.shape[i] - 1) * (size_t)l.strides[i]);
             (reach < 0 ? lo : hi) += reach;
         }
         return std::pair<const char *, const char *>(lo, hi);
@@ -71,6 +74,8 @@ bool rotation(float theta, size_t dh, double *freq_step) {
 
 constexpr size_t MAX_HEAD = 512;         // elements of a head
 constexpr size_t MAX_INDEX = 0x7fffffffu;
+constexpr size_t MAX_TOKENS = 0xffffffu;  // a workgroup of 256 each: a launch has fewer than 2^32 work-items
+constexpr size_t MAX_KEYS = 0x40000000u;  // of a sequence: key numbers and the ends of their tiles fit 31 bits
 
 // ---- the batch: page table [nseq, cols], first tokens [nseq + 1], lengths [nseq], cache [pages, nkvh, page, dh]
 struct BatchMeta {
@@ -101,11 +106,11 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
     const size_t page = static_of(m.page), npages = static_of(m.npages), nseq = static_of(m.nseq);
     if (page == 0) throw shape_not_support("a page of no tokens");
     const size_t cols = npages ? static_of(m.cols) : 0;  // (no pages: no keys)
-    if (nt > MAX_INDEX || nseq >= MAX_INDEX || npages > MAX_INDEX || page > MAX_INDEX || (cols && page > MAX_INDEX / cols))
+    if (nt > MAX_TOKENS || nseq >= MAX_INDEX || npages > MAX_INDEX || page > MAX_KEYS || (cols && page > MAX_KEYS / cols))
         throw shape_not_support("batch or cache too large");
-    expect_strides(table, "page_table");
-    expect_strides(q_start, "q_start");
-    expect_strides(kv_len, "kv_len");
+    expect_static(table, table_base, "page_table");
+    expect_static(q_start, q_start_base, "q_start");
+    expect_static(kv_len, kv_len_base, "kv_len");
     if (!q_start_base || !kv_len_base || (cols && !table_base)) throw args_not_support("null base address");
     PagedBatch b{};
     b.table = table_base;
@@ -178,7 +183,7 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     for (size_t v : {m.nh, m.nt, m.dh, m.nkvh, m.nseq, m.page, m.cols})
         if (is_dyn(v) || v == 0) return a;
     if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || (m.dh != 64 && m.dh != 128) || m.nh % m.nkvh) return a;
-    if (m.nh > MAX_INDEX / m.nt || m.page > MAX_INDEX / m.cols) return a;
+    if (m.nh > MAX_INDEX / m.nt || m.page > MAX_KEYS / m.cols) return a;
     a.matrix = true;
     // Rows per sequence and kv head, on average.  Up to 16: nearly all of it is decode steps.  From 1024 on: 256-row tiles, which
     // load once for twice the rows, and whose last one may stay as empty as it likes (8192 tokens, 32 heads over 8: 558 against
@@ -212,15 +217,14 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     const size_t nh = static_of(m.nh), nt = static_of(m.nt), dh = static_of(m.dh), nkvh = static_of(m.nkvh), nseq = static_of(m.nseq);
     const float scale = static_of(a.scale);
     if (std::isnan(scale) || std::isinf(scale)) throw args_not_support("scale must be a number");
-    expect_strides(a.q_layout, "q");
-    expect_strides(a.o_layout, "o");
-    expect_strides(a.k_cache_layout, "k_cache");
-    expect_strides(a.v_cache_layout, "v_cache");
-    (void)static_of(m.cols), (void)static_of(m.npages), (void)static_of(m.page);
+    expect_static(a.q_layout, a.q_base, "q");
+    expect_static(a.o_layout, a.o_base, "o");
+    expect_static(a.k_cache_layout, a.k_cache_base, "k_cache");
+    expect_static(a.v_cache_layout, a.v_cache_base, "v_cache");
     if (nh == 0 || nt == 0 || dh == 0 || nseq == 0) return;
     AttnPagedParams p{};
     p.b = batch_params(m, nt, a.page_table_layout, a.page_table_base, a.q_start_layout, a.q_start_base, a.kv_len_layout, a.kv_len_base);
-    if (nh > MAX_INDEX / nt) throw shape_not_support("too many rows");
+    if (nh > 0xffffu || nh > MAX_INDEX / nt) throw shape_not_support("too many rows");
     if (!a.q_base || !a.o_base || (p.b.cols && (!a.k_cache_base || !a.v_cache_base))) throw args_not_support("null base address");
     // a workgroup writes rows of o while others still read: o lies apart from what is read, or is q itself, row by row
     if (!same_view(a.o_layout, a.o_base, a.q_layout, a.q_base) && !apart(a.o_layout, a.o_base, a.q_layout, a.q_base))
@@ -241,7 +245,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     p.scale = scale;
     const AttnPagedPlan plan = attention_paged_plan(op, m);
     // (a scale that is not positive: the matrix kernels take the maximum before they scale)
-    if (plan.matrix && p.b.cols && scale > 0.f && plan.grid <= MAX_INDEX && vector_rows(a.q_layout, a.q_base) && vector_rows(a.o_layout, a.o_base) &&
+    if (plan.matrix && p.b.cols && scale > 0.f && plan.grid <= 0xffffffffu / 512 && vector_rows(a.q_layout, a.q_base) && vector_rows(a.o_layout, a.o_base) &&
         vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base)) {
         Workspace ws(qa, workspace, workspace_len, plan.workspace);
         p.work = ws.ptr();
@@ -256,7 +260,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         return;
     }
     op->dev->make_current();
-    launch(op->any[type_index(m.dt)], Dim3{(unsigned)(nt * nh)}, Dim3{256}, 0, stream_of(qa), p);
+    launch(op->any[type_index(m.dt)], Dim3{(unsigned)nt, (unsigned)nh}, Dim3{256}, 0, stream_of(qa), p);
 }
 
 }  // namespace
@@ -331,12 +335,11 @@ void kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_appe
     const size_t nt = static_of(m.nt), dh = static_of(m.dh), nkvh = static_of(m.nkvh), nseq = static_of(m.nseq);
     KvAppendPagedParams p{};
     p.rotate = rotation(a.theta, dh, &p.freq_step);
-    expect_strides(a.k_layout, "k");
-    expect_strides(a.v_layout, "v");
-    expect_strides(a.p_layout, "p");
-    expect_strides(a.k_cache_layout, "k_cache");
-    expect_strides(a.v_cache_layout, "v_cache");
-    (void)static_of(m.cols), (void)static_of(m.npages), (void)static_of(m.page);
+    expect_static(a.k_layout, a.k_base, "k");
+    expect_static(a.v_layout, a.v_base, "v");
+    expect_static(a.p_layout, a.p_base, "p");
+    expect_static(a.k_cache_layout, a.k_cache_base, "k_cache");
+    expect_static(a.v_cache_layout, a.v_cache_base, "v_cache");
     if (nt == 0 || dh == 0 || nkvh == 0 || nseq == 0) return;
     p.b = batch_params(m, nt, a.page_table_layout, a.page_table_base, a.q_start_layout, a.q_start_base, a.kv_len_layout, a.kv_len_base);
     if (p.b.cols == 0) return;  // no place for any key
@@ -450,7 +453,7 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     p.rotate = rotation(a.theta, dh, &p.freq_step);
     p.epsilon = static_of(a.epsilon);
     const ptrdiff_t unit = (ptrdiff_t)ophip_dtype_nbytes(m.dt), wunit = (ptrdiff_t)ophip_dtype_nbytes(m.dt_w);
-    expect_strides(a.p_layout, "p");
+    expect_static(a.p_layout, a.p_base, "p");
     const struct {
         const ophip_tensor_layout &y, &x, &w;
         void *y_base;
@@ -459,9 +462,9 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     } half[2] = {{a.qy_layout, a.q_layout, a.qw_layout, a.qy_base, a.q_base, a.qw_base, nh}, {a.ky_layout, a.k_layout, a.kw_layout, a.ky_base, a.k_base, a.kw_base, nkh}};
     bool vec = dh * unit % 16 == 0;
     for (int i = 0; i < 2; ++i) {
-        expect_strides(half[i].y, "y");
-        expect_strides(half[i].x, "x");
-        expect_strides(half[i].w, "w");
+        expect_static(half[i].y, half[i].y_base, "y");
+        expect_static(half[i].x, half[i].x_base, "x");
+        expect_static(half[i].w, half[i].w_base, "w");
         if (dh && (half[i].y.strides[2] != unit || half[i].x.strides[2] != unit || half[i].w.strides[0] != wunit))
             throw strides_not_support("qk_norm_rope needs a contiguous head dimension");
         p.x[i] = half[i].x_base, p.y[i] = half[i].y_base, p.w[i] = half[i].w_base;
@@ -469,7 +472,7 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
         p.nh[i] = (uint32_t)half[i].nh;
     }
     if (nt == 0 || heads == 0 || dh == 0) return;
-    if (nt > MAX_INDEX || nh > 0xffffu || nkh > 0xffffu) throw shape_not_support("too many tokens or heads");
+    if (nt > MAX_TOKENS || nh > 0xffffu || nkh > 0xffffu) throw shape_not_support("too many tokens or heads");
     for (int i = 0; i < 2; ++i) {
         const auto &h = half[i];
         if (h.nh == 0) continue;

@@ -176,11 +176,68 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
     return true;
 }
 
+// Whether any of a vector's elements is infinite or NaN: its exponent is all ones
+__device__ __forceinline__ uint32_t exponents(uint32_t most, uint32_t pair) {  // the larger of each half, signs aside
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, most), __builtin_bit_cast(u16x2, pair & 0x7fff7fffu)));
+}
+__device__ __forceinline__ bool not_finite(uint32_t most) {
+#ifdef GEMM_ELEM_BF16
+    constexpr uint32_t ONES = 0x7f80u;
+#else
+    constexpr uint32_t ONES = 0x7c00u;
+#endif
+    return (most & 0xffffu) >= ONES || (most >> 16) >= ONES;
+}
+
 // Keys that a row (of the sequence and kv head) keeps
 __device__ __forceinline__ uint32_t paged_keep(const AttnPagedParams &p, const PagedItem &it, uint32_t token) {
     if (!p.causal) return it.s.len;
     const int64_t keep = (int64_t)it.s.len - it.s.n + token + 1;
     return keep < 0 ? 0 : (uint32_t)keep;
+}
+
+// The matrix kernels multiply the values of a tile's keys with a probability of zero where a row does not keep them, and
+// zero times infinity or NaN is NaN.  Where they have met values that are not finite in a tile that some row keeps in part
+// (the last ones under a causal mask), they come here for the whole range instead of handing out their result: a
+// wave to a row, key by key, as in attention_paged_any.hip.  What a row does not keep then does not touch it, whatever it is.
+template <int DH, int ROWS>
+__device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const PagedItem &it, uint32_t key0, uint32_t key1, uint32_t waves) {
+    constexpr int W = DH / WAVE;  // columns per lane
+    const uint32_t lane = threadIdx.x % WAVE;
+    const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 2 * W * lane;
+    const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 2 * W * lane;
+    for (uint32_t r = threadIdx.x / WAVE; r < it.nrows; r += waves) {
+        const uint32_t row = it.row0 + r, token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
+        const elem *qr = reinterpret_cast<const elem *>(reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st) + W * lane;
+        const uint32_t keep = min(key1, paged_keep(p, it, token));
+        float m = -INFINITY, l = 0.f, o[W] = {};
+        for (uint32_t key = key0; key < keep; ++key) {
+            const uint32_t col = fastdiv(key, p.b.page), line = key - col * p.b.page.d, page = min(paged_page(p.b, it.seq, col), p.b.npages - 1);
+            const elem *kr = reinterpret_cast<const elem *>(kb + (int64_t)page * p.k_sp + (int64_t)line * p.k_sr);
+            const elem *vr = reinterpret_cast<const elem *>(vb + (int64_t)page * p.v_sp + (int64_t)line * p.v_sr);
+            float dot = 0.f;
+#pragma unroll
+            for (int i = 0; i < W; ++i) dot += e2f(qr[i]) * e2f(kr[i]);
+            const float x = wave_sum_dpp(dot) * (p.scale * PA_LOG2E), top = fmaxf(m, x);
+            const float old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), e = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top + PA_BIAS);
+            l = l * old + e;
+#pragma unroll
+            for (int i = 0; i < W; ++i) o[i] = o[i] * old + e * e2f(vr[i]);
+            m = top;
+        }
+        if (it.pieces > 1) {
+            float *dst = paged_partial(p, ROWS) + ((size_t)it.slot * ROWS + r) * DH + W * lane;
+#pragma unroll
+            for (int i = 0; i < W; ++i) dst[i] = o[i];
+            if (lane == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + r) * 2) = f32x2{m, l};
+        } else {
+            elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st) + W * lane;
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+            for (int i = 0; i < W; ++i) dst[i] = f2e(o[i] * inv);
+        }
+    }
 }
 
 // ---- up to 16 rows: one pass over the keys at the rate of memory
@@ -204,6 +261,7 @@ struct FewTile {  // 32 keys
 template <int DH>
 struct FewLds {
     float m[4][16], l[4][16], o[4][DH / 4][WAVE];
+    uint32_t bad[4];  // by wave: values that are not finite, in a step that some row keeps in part
 };
 
 // ROWS: of the tiles whose partial results the workspace holds
@@ -259,7 +317,20 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     f32x4 o[CW];
 #pragma unroll
     for (int t = 0; t < CW; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto multiply = [&](const FewTile<CW> &t, uint32_t step) {
+    const uint32_t keep_first = paged_keep(p, it, fastdiv(it.row0, p.group));  // the tile's first row keeps the fewest
+    bool spoiled = false;
+    auto multiply = [&](FewTile<CW> &t, uint32_t step) {
+        if (step * 32 + 32 > keep_first) {  // some rows do not keep some keys
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int d = 0; d < CW / 2; ++d) {
+                    if (step * 32 + 16 * (i / 4) + 4 * g + i % 4 >= it.s.len) t.v[i][d] = 0;  // (the last key again)
+                    most = exponents(most, t.v[i][d]);
+                }
+            spoiled |= __builtin_amdgcn_ballot_w64(not_finite(most)) != 0;
+        }
         float x[8], mx = -INFINITY;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -336,7 +407,9 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
 
     // the four waves' results, on one maximum
     if (g == 0) lds.m[wave][j] = m, lds.l[wave][j] = l;
+    if (lane == 0) lds.bad[wave] = spoiled;
     __syncthreads();
+    if (lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) return paged_exactly<DH, ROWS>(p, it, it.piece * per * 32, last * 32, 4);
     float top = lds.m[0][j];
 #pragma unroll
     for (int w = 1; w < 4; ++w) top = fmaxf(top, lds.m[w][j]);
@@ -398,6 +471,7 @@ struct ManyLds {
     static constexpr int BN = 64;                    // keys of a tile
     static constexpr int KP = DH + 8, VP = DH + 32;  // pitches of a row: reads of consecutive rows spread over the banks
     elem k[2][BN * KP], v[2][BN * VP];
+    uint32_t bad[8];  // by wave: values that are not finite, in a tile that some row keeps in part
 };
 
 template <int DH, int W>
@@ -471,7 +545,20 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             }
         }
     };
-    auto commit = [&](int buf) {
+    const int32_t keep_first = (int32_t)paged_keep(p, it, fastdiv(it.row0, p.group));  // the tile's first row keeps the fewest
+    bool spoiled = false;
+    auto commit = [&](int buf, uint32_t t) {
+        if ((int32_t)(t * BN + BN) > keep_first) {  // some rows do not keep some keys
+            uint32_t most = 0;
+#pragma unroll
+            for (int i = 0; i < NCH; ++i)
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    if (t * BN + cr + RS * i >= it.s.len) vreg[i][d] = 0;  // (the last key again)
+                    most = exponents(most, vreg[i][d]);
+                }
+            spoiled |= __builtin_amdgcn_ballot_w64(not_finite(most)) != 0;
+        }
 #pragma unroll
         for (int i = 0; i < NCH; ++i) {
             st128(&lds.k[buf][(cr + RS * i) * KP + 8 * cc], kreg[i]);
@@ -489,7 +576,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
     if (first < last) {
         look_up(first);
         fetch(first);
-        commit(0);
+        commit(0, first);
         if (first + 1 < last) look_up(first + 1);
     }
 #pragma unroll
@@ -587,9 +674,15 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             }
         }
         __builtin_amdgcn_s_setprio(0);
-        if (more) commit(buf ^ 1);
+        if (more) commit(buf ^ 1, t + 1);
         __syncthreads();
     }
+    if (lane == 0) lds.bad[wave] = spoiled;
+    __syncthreads();
+    uint32_t bad = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) bad |= lds.bad[w];
+    if (bad) return paged_exactly<DH, ROWS>(p, it, first * BN, last * BN, W);
     const float total = l + __shfl_xor(l, 32, WAVE);
     if (wrow + n32 >= it.nrows) return;
     // o[d][4 q + r]: column 32 d + 8 q + 4 h + r of the lane's query

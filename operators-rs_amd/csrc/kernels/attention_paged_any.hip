@@ -13,7 +13,7 @@ template <typename T>
 __device__ __forceinline__ void attn_paged_any(const AttnPagedParams &p) {
     __shared__ float s_m[4], s_l[4], s_o[4][512];
     const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE;
-    const uint32_t nh = p.nkvh * p.group.d, token = blockIdx.x / nh, head = blockIdx.x % nh, kvh = fastdiv(head, p.group);
+    const uint32_t token = blockIdx.x, head = blockIdx.y, kvh = fastdiv(head, p.group);
     const uint32_t seq = paged_seq_of(p.b, token);
     if (seq >= p.b.nseq) return;
     const PagedSeq s = paged_seq(p.b, seq);

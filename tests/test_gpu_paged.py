@@ -138,8 +138,10 @@ class Batch:
 
 
 def check(got, want, tol, what=""):
-    assert np.array_equal(np.isnan(got), np.isnan(want)), what
-    off = np.abs(got - want) - tol
+    """Within the tolerance, and not finite exactly where the definition is not."""
+    fine = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), fine), what
+    off = np.where(fine, np.abs(np.where(fine, got, 0) - np.where(fine, want, 0)) - np.where(fine, tol, 0), 0)
     assert (off <= 0).all(), "%s: %d of %d beyond their tolerance, worst by %g at %s" % (
         what, (off > 0).sum(), off.size, off.max(), np.unravel_index(np.argmax(off), off.shape))
 
@@ -249,7 +251,7 @@ def test_attention_paged_few_and_many_key_ranges(gpu, stream, monkeypatch, tile,
 
 
 @pytest.mark.parametrize("shape", [(4, 2, 64, 16, [(1, 90), (1, 40)]), (4, 2, 128, 16, [(50, 90), (1, 40)])], ids=["few", "many"])
-@pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap", "fused_qkv", "o_over_q", "strided_batch"])
+@pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap", "fused_qkv", "o_over_q", "strided_batch", "unlike_caches", "descending"])
 def test_attention_paged_views(gpu, stream, form, shape):
     """Caches with the tokens of a page in front of the heads, rows farther apart (on 16-byte boundaries and not), q a view of
     a fused projection, o in place of q, and tables and lengths that are views themselves."""
@@ -270,7 +272,18 @@ def test_attention_paged_views(gpu, stream, form, shape):
         t = Buffer(gpu, np.repeat(np.repeat(b.table.host, 2, 0), 3, 1)[::-1, ::-1])
         st, ln = Buffer(gpu, np.repeat(b.q_start.host, 2)), Buffer(gpu, b.kv_len.host[::-1].astype(np.int32))
         batch = t.view(t.host[::-1, ::-1][::2, ::3]) + st.view(st.host[::2]) + ln.view(ln.host[::-1])
-    run(gpu, stream, ophip.AttentionPagedArgs(*qa, *b.cache_args(), *oa, *batch, 1, scale))
+    caches = b.cache_args()
+    if form == "unlike_caches":  # v with a page's tokens in front of its heads
+        v = Buffer(gpu, b.cache[1].host.swapaxes(1, 2), "f16")
+        caches = b.cache[0].view() + v.view(v.host.swapaxes(1, 2))
+    if form == "descending":  # pages, heads, tokens, q and o in descending order of addresses
+        flipped = [Buffer(gpu, c.host[::-1, ::-1, ::-1], "f16") for c in b.cache]
+        caches = flipped[0].view(flipped[0].host[::-1, ::-1, ::-1]) + flipped[1].view(flipped[1].host[::-1, ::-1, ::-1])
+        qf, of = Buffer(gpu, b.q.host[::-1], "f16"), Buffer(gpu, b.o.host[:, ::-1], "f16")
+        qa, oa = qf.view(qf.host[::-1].transpose(1, 0, 2)), of.view(of.host[:, ::-1].transpose(1, 0, 2))
+    run(gpu, stream, ophip.AttentionPagedArgs(*qa, *caches, *oa, *batch, 1, scale))
+    if form == "descending":
+        return check(decode(of.back(stream)[:, ::-1], "f16"), want, tol)
     got = b.q.back(stream) if form == "o_over_q" else b.o.back(stream)
     check(decode(got, "f16"), want, tol)
 
@@ -289,6 +302,30 @@ def test_attention_paged_one_key_outweighs_the_others(gpu, stream, lens):
     b.q = Buffer(gpu, (b.q.host * np.float16(20)).astype(np.float16), "f16")
     want, tol = b.expected(1)
     check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+@pytest.mark.parametrize("kind,value", [("f16", np.nan), ("bf16", np.inf)])
+@pytest.mark.parametrize("dh", [64, 128, 40])
+def test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, tile, kind, value, dh):
+    """Keys and values that are not finite spoil the rows that see them, wherever the mask ends, and no other."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(19), kind, 4, 2, dh, 16, [(40, 90), (3, 70), (1, 130), (300, 300), (5, 3)])
+    bits = lambda x: encode(np.array([x]), kind)[0]
+
+    def put(which, s, key, head, col):
+        b.cache_views[which][b.table.host[s, key // 16], head, key % 16, col] = bits(value)
+
+    put(1, 0, 75, 0, 3), put(1, 0, 89, 1, 5), put(1, 1, 69, 0, 0), put(1, 1, 68, 1, dh - 1)
+    put(1, 2, 129, 0, 7), put(1, 3, 130, 1, 8), put(1, 3, 200, 0, 1), put(1, 3, 250, 0, 2), put(0, 3, 290, 1, 4), put(1, 4, 1, 0, 6)
+    b.cache = [Buffer(gpu, c.host, kind) for c in b.cache]
+    b.cache_views = [c.host for c in b.cache]
+    for mask in (1, 0):
+        gpu.upload(b.o.mem, b.o.host)
+        with np.errstate(invalid="ignore"):
+            want, tol = b.expected(mask)
+        assert not np.isfinite(want).all() and np.isfinite(want).any()
+        check(attend(gpu, stream, b, mask), want, tol, "mask %d" % mask)
 
 
 @pytest.mark.parametrize("lens", [[(1, 50), (1, 300), (1, 9)], [(40, 60), (1, 300), (20, 20)]], ids=["few", "many"])
@@ -394,6 +431,10 @@ def test_attention_paged_refusals(gpu, stream):
         refused("ArgsNotSupport", at_scheme=False, **{n: None})
     refused("ArgsNotSupport", at_scheme=False, o_base=good.q_base + 64)        # o part over q
     refused("ArgsNotSupport", at_scheme=False, o_base=good.k_cache_base)
+    refused("ArgsNotSupport", at_scheme=False, kv_len_base=good.kv_len_base + 2)
+    refused("ArgsNotSupport", at_scheme=False, q_base=good.q_base + 1)
+    refused("ShapeNotSupport", at_scheme=False, page_table_layout=L(good.page_table_layout, shape=[2, 1 << 28]))  # 2^32 keys
+    refused("DynamicNotSupport", at_scheme=False, q_layout=L(good.q_layout, shape=[None, 3, 64]))
     dyn = L(good.q_layout, strides=[None, None, None])
     dyn_args = b.args(1)
     dyn_args.q_layout = dyn
