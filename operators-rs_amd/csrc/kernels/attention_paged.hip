@@ -78,8 +78,9 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
     const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE, w = blockIdx.x;
     uint32_t local, first_slot;
     if (p.b.nseq <= WAVE) {
-        // A sequence per lane, each wave for itself.  The longest come first: the units that end last should not also
-        // begin last.
+        // A sequence per lane, and the longest first: the units that end last should not also begin last.  So what comes before
+        // a sequence is a sum over all others, of which each wave takes its share.
+        __shared__ uint32_t s_before[2][WAVES][WAVE], s_all[WAVES];
         const bool on = lane < p.b.nseq;
         PagedSeq s{0, 0, 0};
         if (on) s = paged_seq(p.b, lane);
@@ -88,13 +89,19 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         const uint32_t pieces = paged_pieces<ROWS>(p, s, paged_per_step(p, work));
         const uint32_t items = tiles * p.nkvh * pieces, slots = pieces > 1 ? items : 0;
         uint32_t items0 = 0, slots0 = 0, all_slots = 0;
-        for (uint32_t k = 0; k < p.b.nseq; ++k) {
+        for (uint32_t k = wave; k < p.b.nseq; k += WAVES) {
             const uint32_t len = __builtin_amdgcn_readlane(s.len, k), ni = __builtin_amdgcn_readlane(items, k), ns = __builtin_amdgcn_readlane(slots, k);
             const bool before = len > s.len || (len == s.len && k < lane);
             items0 += before ? ni : 0;
             slots0 += before ? ns : 0;
             all_slots += ns;
         }
+        s_before[0][wave][lane] = items0, s_before[1][wave][lane] = slots0;
+        if (lane == 0) s_all[wave] = all_slots;
+        __syncthreads();
+        items0 = slots0 = all_slots = 0;
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) items0 += s_before[0][v][lane], slots0 += s_before[1][v][lane], all_slots += s_all[v];
         if (w == 0 && tid == 0 && p.slots) *reinterpret_cast<uint32_t *>(p.work) = min(all_slots, p.slots);
         const uint64_t mine = __builtin_amdgcn_ballot_w64(w - items0 < items);
         if (mine == 0) return false;
@@ -695,19 +702,21 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
         if (h == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + at) * 2) = f32x2{m, total};
         return;
     }
+    // two quads of a query are adjacent in lanes l and l + 32: one of each pair goes over, so that a lane stores 16 bytes
     const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
-    char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 8 * h;
+    char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 16 * h;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < 4; q += 2) {
             union {
-                elem e[4];
-                u32x2 u;
+                elem e[8];
+                uint32_t u[4];
             } y;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) y.e[r] = f2e(o[d][4 * q + r] * inv);
-            *reinterpret_cast<u32x2 *>(dst + 64 * d + 16 * q) = y.u;
+            for (int r = 0; r < 8; ++r) y.e[r] = f2e(o[d][4 * q + r] * inv);
+            const uint32_t s0 = __shfl_xor(h ? y.u[0] : y.u[2], 32, WAVE), s1 = __shfl_xor(h ? y.u[1] : y.u[3], 32, WAVE);
+            st128(dst + 64 * d + 16 * q, h ? u32x4{s0, s1, y.u[2], y.u[3]} : u32x4{y.u[0], y.u[1], s0, s1});
         }
 }
 
