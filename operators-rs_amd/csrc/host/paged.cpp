@@ -128,9 +128,9 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 
 struct ophip_attention_paged : OpBase {
     hipFunction_t any[3];
-    hipFunction_t rows[2][3][2], join[2][3][2];  // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64 / 128]
+    hipFunction_t rows[2][3][2], join[2][3][2];  // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64 / 128], 256 for dh 128 only
     // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2
-    // one size of tile
+    // one size of tile (2: 1 where dh is 64)
     int slots = 0, tile = -1;
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
         any[0] = d->kernel("attention_paged_any", "attn_paged_any_f16");
@@ -138,7 +138,7 @@ struct ophip_attention_paged : OpBase {
         any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
         for (int e = 0; e < 2; ++e)
             for (int r = 0; r < 3; ++r)
-                for (int h = 0; h < 2; ++h) {
+                for (int h = r == 2; h < 2; ++h) {
                     const char *mod = e ? "attention_paged_bf16" : "attention_paged";
                     const std::string tail = std::string(r == 0 ? "few" : r == 1 ? "many" : "wide") + (h ? "_d128" : "_d64") + (e ? "_bf16" : "");
                     rows[e][r][h] = d->kernel(mod, ("attn_paged_" + tail).c_str());
@@ -185,12 +185,18 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || (m.dh != 64 && m.dh != 128) || m.nh % m.nkvh) return a;
     if (m.nh > MAX_INDEX / m.nt || m.page > MAX_KEYS / m.cols) return a;
     a.matrix = true;
-    // Rows per sequence and kv head, on average.  Up to 16: nearly all of it is decode steps.  From 1024 on: 256-row tiles, which
-    // load once for twice the rows, and whose last one may stay as empty as it likes (8192 tokens, 32 heads over 8: 558 against
-    // 585 us, 511 tokens over 32511 keys 299 against 318; prompts of 104 .. 546 tokens 36.8 against 32.6).
-    const size_t group = m.nh / m.nkvh, rows = m.nt * group;
-    a.tile = rows <= 16 * m.nseq ? 0 : rows < 1024 * m.nseq ? 1 : 2;
-    if (op && op->tile >= 0 && op->tile <= 2) a.tile = op->tile;
+    const size_t cus = (size_t)(op ? op->dev->props.multiProcessorCount : 256);
+    // Tiles of 16 rows where nearly all sequences have no more, and where there is little to do: a tile of 128 rows then takes
+    // its keys with fewer workgroups than there are CUs (403 tokens of 12 sequences, 4 heads over 2, up to 2035 keys: 14.0
+    // against 17.5 us; 127 tokens of 2 sequences, 16 heads over 8, 5479 keys, over twice the bound: 57 against 26.5; 280 tokens
+    // of 2 sequences, 64 heads over 32, 161 keys, twice the bound of rows: 11.5 against 8.5).
+    // Tiles of 256, which load once for twice the rows, where a sequence fills several and the work is long (8192 tokens,
+    // 32 heads over 8: 558 against 585 us, 511 tokens over 32511 keys 299 against 318; shorter than the bound, 7 prompts of up
+    // to 546 tokens 36.8 against 32.6; dh 64 never gains by them).
+    const size_t group = m.nh / m.nkvh, rows = m.nt * group, products = m.nkvh * rows * (m.page * m.cols);  // (below 2^61)
+    if ((products <= cus << 14 && m.nkvh * rows <= cus << 5) || (group <= 16 && m.nt <= 2 * m.nseq)) a.tile = 0;
+    else a.tile = m.dh == 128 && rows >= 1024 * m.nseq && products >= cus << 20 ? 2 : 1;
+    if (op && op->tile >= 0 && op->tile <= 2) a.tile = m.dh == 128 ? op->tile : std::min(op->tile, 1);
     const size_t tile = a.tile == 0 ? 16 : a.tile == 1 ? 128 : 256;
     // the most tiles there can be, whatever the lengths: each sequence that has a token may have one that is not full
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
@@ -200,7 +206,6 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     // 32511 keys, 32 heads over 8, on tiles of 128: 420 us with half as many, 321, 338 with twice as many), and four per CU
     // for 16 rows, where a range costs little and the rates of memory even out (50 decode steps over 165008 keys: 134 us
     // with 512, 122 with 1024, 124 with 1536).
-    const size_t cus = (size_t)(op ? op->dev->props.multiProcessorCount : 256);
     const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 ? 2 : 1) * cus;
     a.grid = units;
     if (most > 1) {
@@ -250,6 +255,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         Workspace ws(qa, workspace, workspace_len, plan.workspace);
         p.work = ws.ptr();
         p.slots = (uint32_t)plan.slots;
+        p.cus = (uint32_t)(op->slots > 0 ? op->slots : op->dev->props.multiProcessorCount);
         const ptrdiff_t far = (ptrdiff_t)1 << 31;
         p.narrow = p.k_sp == p.v_sp && p.k_sr == p.v_sr && p.k_sp >= 0 && p.k_sp < far && p.k_sr >= 0 && p.k_sr < far / (ptrdiff_t)p.b.page.d &&
                    p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;

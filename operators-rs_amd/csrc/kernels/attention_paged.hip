@@ -66,10 +66,15 @@ __device__ __forceinline__ uint32_t paged_pieces(const AttnPagedParams &p, const
     const uint32_t most = paged_steps(s) / least;
     return p.slots && most > 1 ? min(most, max(1u, (uint32_t)(paged_weight(p, s) * per_step + 0.5f))) : 1;
 }
-// `work`: tiles times weight of all sequences.  Three quarters of the slots: a count rounded to two or more is at most four
-// thirds of what it was.
+// Ranges per unit of weight.  `work`: tiles times weight of all sequences.  As many as there are slots (three quarters: a count
+// rounded to two or more is at most four thirds of what it was) for long batches, but beyond one per CU only while each has
+// 24 steps of its own, or 8 of a tile that weighs twice: the plan, the first loads and the join cost as much as several
+// steps (31 decode steps over 57 MB in 1024 / 512 / 256 ranges: 27.9 / 19.4 / 17.5 us).
+template <int ROWS>
 __device__ __forceinline__ float paged_per_step(const AttnPagedParams &p, float work) {
-    return work > 0.f ? 0.74999f * (float)p.slots / (work * (float)p.nkvh) : 0.f;
+    if (!(work > 0.f)) return 0.f;
+    const float all = work * (float)p.nkvh;
+    return fminf(0.74999f * (float)p.slots, fmaxf((float)p.cus, all * (1.f / (ROWS == FEW ? 24.f : 16.f)))) / all;
 }
 
 // What workgroup blockIdx.x does; false: nothing.  Every thread calls it and gets the same.
@@ -86,7 +91,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
         if (on) s = paged_seq(p.b, lane);
         const uint32_t tiles = paged_tiles<ROWS>(p, s);
         const float work = p.slots ? wave_sum_dpp((float)tiles * paged_weight(p, s)) : 0.f;
-        const uint32_t pieces = paged_pieces<ROWS>(p, s, paged_per_step(p, work));
+        const uint32_t pieces = paged_pieces<ROWS>(p, s, paged_per_step<ROWS>(p, work));
         const uint32_t items = tiles * p.nkvh * pieces, slots = pieces > 1 ? items : 0;
         uint32_t items0 = 0, slots0 = 0, all_slots = 0;
         for (uint32_t k = wave; k < p.b.nseq; k += WAVES) {
@@ -131,7 +136,7 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
             float work = 0.f;
 #pragma unroll
             for (int v = 0; v < WAVES; ++v) work += s_work[v];
-            per_step = paged_per_step(p, work);
+            per_step = paged_per_step<ROWS>(p, work);
         }
         uint32_t items0 = 0, slots0 = 0;
         for (uint32_t i0 = 0; i0 < p.b.nseq; i0 += THREADS) {
@@ -799,12 +804,13 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     } else paged_many<DH, W>(p, it, lds.many);
 }
 
-#define ATTN_PAGED(DH)                                                                                                                                   \
-    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_few_d##DH)(AttnPagedParams p) { attn_paged_few<DH>(p); }                  \
-    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 4>(p); }             \
-    extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 8>(p); }             \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 16>(p); }           \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }         \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 256>(p); }
+#define ATTN_PAGED(DH)                                                                                                                        \
+    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_few_d##DH)(AttnPagedParams p) { attn_paged_few<DH>(p); }       \
+    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 4>(p); }  \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 16>(p); } \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }
 ATTN_PAGED(64)
 ATTN_PAGED(128)
+// (dh 64 gains nothing by tiles of 256: 8192 tokens, 32 heads over 8, 391 against 363 us)
+extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8>(p); }
+extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256>(p); }

@@ -289,6 +289,7 @@ struct AttnPagedParams {
     FastDivU32 group;  // query heads per kv head
     uint32_t nkvh, dh, causal;
     uint32_t slots;     // key ranges the work area holds, and the number that the tiles are split into together; 0: no splitting
+    uint32_t cus;       // as many key ranges are made of short batches, too
     uint32_t narrow;  // both caches of one layout, and distances inside a page, a row of the table and from page to page of less than 32 bits
     float scale;
 };
