@@ -495,10 +495,14 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
     const size_t vectors = dh * unit / 16;
     vec = vec && vectors <= 64;
     const int li = vectors <= 8 ? 0 : vectors <= 16 ? 1 : vectors <= 32 ? 2 : 3;
-    // Few tokens: a token's heads over several workgroups, down to one row for each group of lanes.  Many: several tokens to
-    // a workgroup, two pairs of sine and cosine for each of its 256 threads.  Stores are non-temporal where
+    // Few tokens: a token's heads over several workgroups, down to one row for each group of lanes.  More: up to eight tokens to
+    // a workgroup, so that its 256 threads share the sines and cosines, two pairs for each at the most; as many as its four
+    // rows per thread hold, or more where that still leaves two workgroups per CU (16 + 2 heads of 128, tokens with 1 / 2 / 4 / 8
+    // to a workgroup: 512 10.1 / 6.9 / 7.8 / 9.9 us, 2048 19.3 / 12.7 / 10.7 / 11.3, 4095 34.1 / 21.1 / 16.5 / 15.6;
+    // 36 + 12 heads, 2048 21.7 / 17.3 / 17.3 / 20.9; 4 + 1 heads, 2048 17.1 / 10.1 / 7.8 / 6.5).  Stores are non-temporal where
     // the result is larger than the L2 caches together (8 x 4 MiB): whoever reads it next does not find it there.
-    const size_t rows = vec ? 32u >> li : 4, tokens = vec && nt >= 4096 ? std::max<size_t>(1, 1024 / dh) : 1;
+    const size_t rows = vec ? 32u >> li : 4, fit = nt < 256 ? 1 : 4 * rows / heads, full = nt < 512 ? 1 : nt < 2048 ? 2 : nt < 4096 ? 4 : 8;
+    const size_t tokens = vec ? std::max<size_t>(1, std::min({std::max(fit, full), (size_t)8, 1024 / dh})) : 1;
     const size_t by = tokens > 1 ? 1 : std::min((heads + rows - 1) / rows, std::max<size_t>(1, 1024 / nt)), per = (heads + by - 1) / by;
     p.heads_per_block = make_fastdiv((uint32_t)per);
     p.tokens_per_block = (uint32_t)tokens;

@@ -1,6 +1,6 @@
 // qk_norm_rope: y = rope(x / sqrt(mean(x^2) + epsilon) * w, p) for every head of q and of k, in one pass and one launch.
 //
-// A workgroup serves some consecutive tokens, or one slice of one token's nh + nkh heads when there are few.  A row (one
+// A workgroup serves up to eight consecutive tokens, or one slice of one token's nh + nkh heads when there are few.  A row (one
 // head) is 16 bytes in each of L consecutive lanes, so its sum of squares is a sum over L lanes and everything else stays
 // in the lane: each byte is read once and written once, and what bounds the kernel is memory.  The tokens' sines and
 // cosines are evaluated once into LDS, a pair of a token per thread, while the first rows travel (an evaluation is some fifty

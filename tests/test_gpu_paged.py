@@ -788,3 +788,58 @@ def test_null_operators_and_arguments(gpu):
         assert getattr(L, "ophip_%s_launch" % n)(None, None, None, ctypes.c_size_t(0), None) == 8
         assert getattr(L, "ophip_%s_scheme" % n)(None, None, ctypes.c_size_t(0), ctypes.byref(ws)) == 8
         getattr(L, "ophip_%s_destroy" % n)(None)
+
+
+# ---- what the choice of tile by size would leave out: each batch on the tiles that others of its kind have
+
+TILED = [s for s in SHAPES if s[2] in (64, 128)]
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("shape", TILED, ids=lambda s: "%d-%d-%d-%d-%s" % (s[0], s[1], s[2], s[3], "_".join("%dof%d" % x for x in s[4])))
+def test_attention_paged_shapes_on_every_tile(gpu, stream, monkeypatch, shape, kind, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged(gpu, stream, shape, 1, kind)
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+@pytest.mark.parametrize("form", ["token_major", "head_gap", "odd_gap", "fused_qkv", "o_over_q", "strided_batch", "unlike_caches", "descending"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_views_on_every_tile(gpu, stream, monkeypatch, form, dh, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged_views(gpu, stream, form, (4, 2, dh, 16, [(50, 90), (1, 40), (3, 3)]))
+
+
+@pytest.mark.parametrize("tile", ["1", "2"])
+def test_attention_paged_hard_batches_on_large_tiles(gpu, stream, monkeypatch, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged_one_key_outweighs_the_others(gpu, stream, [(40, 60), (1, 300)])
+    test_attention_paged_offsets_past_32_bits(gpu, stream)
+    test_attention_paged_recorded_and_replayed_with_other_lengths(gpu, stream, 12)
+    for lens in ([(1, 50), (1, 300), (1, 9)], [(40, 60), (1, 300), (20, 20)]):
+        test_attention_paged_bad_descriptions_stay_inside(gpu, stream, lens, 64)
+
+
+@pytest.mark.parametrize("tile", ["0", "1"])
+@pytest.mark.parametrize("count", [65, 600])
+def test_attention_paged_many_sequences_on_every_tile(gpu, stream, monkeypatch, count, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged_many_sequences(gpu, stream, count, 2)
+
+
+@pytest.mark.parametrize("lens,nh,nkvh", [([(600, 600), (3, 900)], 4, 4), ([(2, 700)] * 5 + [(40, 300)], 16, 2), ([(1, 260)] * 40, 16, 8), ([(1200, 1200)], 8, 1)],
+                         ids=["prompt", "chunks", "decode", "long"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_sizes_between_the_kernels(gpu, stream, lens, nh, nkvh, dh):
+    """On the tiles that the sizes choose, with ranges cut for one workgroup per CU and for more."""
+    b = Batch(gpu, np.random.default_rng(41), "bf16", nh, nkvh, dh, 16, lens, pad=2)
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("nt,nh,nkh,dh", [(255, 2, 1, 64), (256, 2, 1, 64), (257, 4, 4, 128), (511, 6, 2, 128), (513, 6, 2, 128), (1029, 17, 3, 64), (2049, 5, 2, 128),
+                                          (2051, 1, 0, 8), (300, 0, 3, 512), (600, 65, 1, 96)])
+def test_qk_norm_rope_two_four_and_eight_tokens_per_workgroup(gpu, stream, nt, nh, nkh, dh):
+    check_norm(gpu, stream, np.random.default_rng(42), nt, nh, nkh, dh, "f16", "f32", 10000.0)
+    check_norm(gpu, stream, np.random.default_rng(43), nt, nh, nkh, dh, "bf16", "bf16", 0.0)
