@@ -128,7 +128,8 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 
 struct ophip_attention_paged : OpBase {
     hipFunction_t any[3];
-    hipFunction_t rows[2][3][2], join[2][3][2];  // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64 / 128], 256 for dh 128 only
+    // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64, 128, below 64, below 128, up to 256]; 256 rows for dh 128 only
+    hipFunction_t rows[2][3][5], join[2][3][5];
     // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2
     // one size of tile (2: 1 where dh is 64)
     int slots = 0, tile = -1;
@@ -138,9 +139,11 @@ struct ophip_attention_paged : OpBase {
         any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
         for (int e = 0; e < 2; ++e)
             for (int r = 0; r < 3; ++r)
-                for (int h = r == 2; h < 2; ++h) {
+                for (int h = 0; h < 5; ++h) {
+                    if (r == 2 && h != 1) continue;
+                    static const char *const head[5] = {"d64", "d128", "d64_pad", "d128_pad", "d256_pad"};
                     const char *mod = e ? "attention_paged_bf16" : "attention_paged";
-                    const std::string tail = std::string(r == 0 ? "few" : r == 1 ? "many" : "wide") + (h ? "_d128" : "_d64") + (e ? "_bf16" : "");
+                    const std::string tail = std::string(r == 0 ? "few_" : r == 1 ? "many_" : "wide_") + head[h] + (e ? "_bf16" : "");
                     rows[e][r][h] = d->kernel(mod, ("attn_paged_" + tail).c_str());
                     join[e][r][h] = d->kernel(mod, ("attn_paged_join_" + tail).c_str());
                 }
@@ -174,7 +177,7 @@ AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
 // How the matrix kernels take a call (attention_paged.hip), from its sizes alone.
 struct AttnPagedPlan {
     bool matrix;                    // they serve these types and sizes
-    int tile;                       // tiles of 16, 128 or 256 rows: 0, 1, 2
+    int tile, head;                 // tiles of 16, 128 or 256 rows: 0, 1, 2; of the kernels' head dimensions
     size_t grid, slots;  // workgroups; key ranges the workspace holds (0: no tile can be cut)
     size_t workspace;
 };
@@ -182,9 +185,11 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     AttnPagedPlan a{};
     for (size_t v : {m.nh, m.nt, m.dh, m.nkvh, m.nseq, m.page, m.cols})
         if (is_dyn(v) || v == 0) return a;
-    if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || (m.dh != 64 && m.dh != 128) || m.nh % m.nkvh) return a;
+    if ((m.dt != OPHIP_DT_F16 && m.dt != OPHIP_DT_BF16) || m.dh % 8 || m.dh > 256 || m.nh % m.nkvh) return a;
     if (m.nh > MAX_INDEX / m.nt || m.page > MAX_KEYS / m.cols) return a;
     a.matrix = true;
+    a.head = m.dh == 64 ? 0 : m.dh == 128 ? 1 : m.dh < 64 ? 2 : m.dh < 128 ? 3 : 4;
+    const size_t dh = m.dh <= 64 ? 64 : m.dh <= 128 ? 128 : 256;  // columns that they work on
     const size_t cus = (size_t)(op ? op->dev->props.multiProcessorCount : 256);
     // Tiles of 16 rows where nearly all sequences have no more, and where there is little to do: a tile of 128 rows then takes
     // its keys with fewer workgroups than there are CUs (403 tokens of 12 sequences, 4 heads over 2, up to 2035 keys: 14.0
@@ -211,7 +216,7 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     if (most > 1) {
         a.slots = std::min((4 * want + 2) / 3, units * most);
         a.grid = std::min(units * most, units + (4 * want + 2) / 3);
-        a.workspace = 64 + a.slots * (32 + tile * (m.dh + 2) * sizeof(float));
+        a.workspace = 64 + a.slots * (32 + tile * (dh + 2) * sizeof(float));
     }
     return a;
 }
@@ -259,7 +264,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         const ptrdiff_t far = (ptrdiff_t)1 << 31;
         p.narrow = p.k_sp == p.v_sp && p.k_sr == p.v_sr && p.k_sp >= 0 && p.k_sp < far && p.k_sr >= 0 && p.k_sr < far / (ptrdiff_t)p.b.page.d &&
                    p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;
-        const int e = m.dt == OPHIP_DT_BF16, h = dh == 128;
+        const int e = m.dt == OPHIP_DT_BF16, h = plan.head;
         op->dev->make_current();
         launch(op->rows[e][plan.tile][h], Dim3{(unsigned)plan.grid}, Dim3{plan.tile == 2 ? 512u : 256u}, 0, stream_of(qa), p);
         if (plan.slots) launch(op->join[e][plan.tile][h], Dim3{(unsigned)plan.slots}, Dim3{256}, 0, stream_of(qa), p);

@@ -213,15 +213,17 @@ __device__ __forceinline__ uint32_t paged_keep(const AttnPagedParams &p, const P
 // zero times infinity or NaN is NaN.  Where they have met values that are not finite in a tile that some row keeps in part
 // (the last ones under a causal mask), they come here for the whole range instead of handing out their result: a
 // wave to a row, key by key, as in attention_paged_any.hip.  What a row does not keep then does not touch it, whatever it is.
-template <int DH, int ROWS>
+template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const PagedItem &it, uint32_t key0, uint32_t key1, uint32_t waves) {
     constexpr int W = DH / WAVE;  // columns per lane
     const uint32_t lane = threadIdx.x % WAVE;
-    const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 2 * W * lane;
-    const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 2 * W * lane;
+    const bool live = !PAD || W * lane < p.dh;  // (the others: column 0 again, of no weight and not stored)
+    const uint32_t c0 = live ? W * lane : 0;
+    const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 2 * c0;
+    const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 2 * c0;
     for (uint32_t r = threadIdx.x / WAVE; r < it.nrows; r += waves) {
         const uint32_t row = it.row0 + r, token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
-        const elem *qr = reinterpret_cast<const elem *>(reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st) + W * lane;
+        const elem *qr = reinterpret_cast<const elem *>(reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st) + c0;
         const uint32_t keep = min(key1, paged_keep(p, it, token));
         float m = -INFINITY, l = 0.f, o[W] = {};
         for (uint32_t key = key0; key < keep; ++key) {
@@ -230,7 +232,7 @@ __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const Pa
             const elem *vr = reinterpret_cast<const elem *>(vb + (int64_t)page * p.v_sp + (int64_t)line * p.v_sr);
             float dot = 0.f;
 #pragma unroll
-            for (int i = 0; i < W; ++i) dot += e2f(qr[i]) * e2f(kr[i]);
+            for (int i = 0; i < W; ++i) dot += live ? e2f(qr[i]) * e2f(kr[i]) : 0.f;
             const float x = wave_sum_dpp(dot) * (p.scale * PA_LOG2E), top = fmaxf(m, x);
             const float old = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - top), e = x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x - top + PA_BIAS);
             l = l * old + e;
@@ -238,13 +240,14 @@ __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const Pa
             for (int i = 0; i < W; ++i) o[i] = o[i] * old + e * e2f(vr[i]);
             m = top;
         }
+        if (!live) continue;
         if (it.pieces > 1) {
-            float *dst = paged_partial(p, ROWS) + ((size_t)it.slot * ROWS + r) * DH + W * lane;
+            float *dst = paged_partial(p, ROWS) + ((size_t)it.slot * ROWS + r) * DH + c0;
 #pragma unroll
             for (int i = 0; i < W; ++i) dst[i] = o[i];
             if (lane == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + r) * 2) = f32x2{m, l};
         } else {
-            elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st) + W * lane;
+            elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st) + c0;
             const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
             for (int i = 0; i < W; ++i) dst[i] = f2e(o[i] * inv);
@@ -277,7 +280,7 @@ struct FewLds {
 };
 
 // ROWS: of the tiles whose partial results the workspace holds
-template <int DH, int ROWS>
+template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedItem &it, FewLds<DH> &lds) {
     constexpr int CW = DH / 16, KS = DH / 32;  // columns of v per lane, contraction steps of q . k
     const uint32_t wave = threadIdx.x / WAVE, lane = threadIdx.x % WAVE, j = lane % 16, g = lane / 16;
@@ -290,7 +293,7 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     {
         const char *src = reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st + 16 * g;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = ld128(src + 64 * s);
+        for (int s = 0; s < KS; ++s) q[s] = !PAD || 32 * s + 8 * g < p.dh ? ld128(src + 64 * s) : u32x4{0, 0, 0, 0};
     }
     const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 16 * g;
     const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 2 * CW * j;
@@ -312,7 +315,7 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
             pg[c] = min(page[c], p.b.npages - 1);
             const char *src = kb + (int64_t)pg[c] * p.k_sp + (int64_t)line[c] * p.k_sr;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) t.k[c][s] = ld128_nt(src + 64 * s);
+            for (int s = 0; s < KS; ++s) t.k[c][s] = !PAD || 32 * s + 8 * g < p.dh ? ld128_nt(src + 64 * s) : u32x4{0, 0, 0, 0};
         }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
@@ -320,8 +323,13 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
             for (int i = 0; i < 4; ++i) {
                 const uint32_t vp = __shfl(pg[c], 4 * g + i, WAVE), vl = __shfl(line[c], 4 * g + i, WAVE);
                 const char *src = vb + (int64_t)vp * p.v_sp + (int64_t)vl * p.v_sr;
-                if constexpr (CW == 8) *reinterpret_cast<u32x4 *>(t.v[4 * c + i]) = ld128_nt(src);
-                else *reinterpret_cast<u32x2 *>(t.v[4 * c + i]) = __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src));
+                if constexpr (CW == 4) {
+                    *reinterpret_cast<u32x2 *>(t.v[4 * c + i]) = !PAD || CW * j < p.dh ? __builtin_nontemporal_load(reinterpret_cast<const u32x2 *>(src)) : u32x2{0, 0};
+                } else {
+#pragma unroll
+                    for (int w = 0; w < CW; w += 8)
+                        *reinterpret_cast<u32x4 *>(t.v[4 * c + i] + w / 2) = !PAD || CW * j + w < p.dh ? ld128_nt(src + 2 * w) : u32x4{0, 0, 0, 0};
+                }
             }
     };
     const float scale2 = p.scale * PA_LOG2E;
@@ -421,7 +429,7 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     if (g == 0) lds.m[wave][j] = m, lds.l[wave][j] = l;
     if (lane == 0) lds.bad[wave] = spoiled;
     __syncthreads();
-    if (lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) return paged_exactly<DH, ROWS>(p, it, it.piece * per * 32, last * 32, 4);
+    if (lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3]) return paged_exactly<DH, ROWS, PAD>(p, it, it.piece * per * 32, last * 32, 4);
     float top = lds.m[0][j];
 #pragma unroll
     for (int w = 1; w < 4; ++w) top = fmaxf(top, lds.m[w][j]);
@@ -454,14 +462,18 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
     union {
         elem e[CW];
-        u32x4 u4;
-        u32x2 u2;
+        uint32_t u[CW / 2];
     } y;
 #pragma unroll
     for (int t = 0; t < CW; ++t) y.e[t] = f2e(out[t] * inv);
     char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 2 * column;
-    if constexpr (CW == 8) st128(dst, y.u4);
-    else *reinterpret_cast<u32x2 *>(dst) = y.u2;
+    if constexpr (CW == 4) {
+        if (!PAD || column < p.dh) *reinterpret_cast<u32x2 *>(dst) = u32x2{y.u[0], y.u[1]};
+    } else {
+#pragma unroll
+        for (int w = 0; w < CW; w += 8)
+            if (!PAD || column + w < p.dh) st128(dst + 2 * w, u32x4{y.u[w / 2], y.u[w / 2 + 1], y.u[w / 2 + 2], y.u[w / 2 + 3]});
+    }
 }
 
 // ---- up to 128 rows: the products are the work
@@ -486,7 +498,7 @@ struct ManyLds {
     uint32_t bad[8];  // by wave: values that are not finite, in a tile that some row keeps in part
 };
 
-template <int DH, int W>
+template <int DH, int W, bool PAD>
 __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const PagedItem &it, ManyLds<DH> &lds) {
     constexpr int BN = ManyLds<DH>::BN, KP = ManyLds<DH>::KP, VP = ManyLds<DH>::VP;
     constexpr int CPR = DH / 8, ROWS = 32 * W, NCH = BN * CPR / (W * WAVE), RS = W * WAVE / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
@@ -506,9 +518,10 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
     {
         const char *src = reinterpret_cast<const char *>(p.q) + (int64_t)head * p.q_sh + (int64_t)(it.s.start + token) * p.q_st + 16 * h;
 #pragma unroll
-        for (int d = 0; d < DS; ++d) qf[d].u = ld128(src + 32 * d);
+        for (int d = 0; d < DS; ++d) qf[d].u = !PAD || 16 * d + 8 * h < p.dh ? ld128(src + 32 * d) : u32x4{0, 0, 0, 0};
     }
     const uint32_t cc = tid % CPR, cr = tid / CPR;
+    const bool live = !PAD || 8 * cc < p.dh;
     const char *kb = reinterpret_cast<const char *>(p.k) + (int64_t)it.kvh * p.k_sh + 16 * cc;
     const char *vb = reinterpret_cast<const char *>(p.v) + (int64_t)it.kvh * p.v_sh + 16 * cc;
     uint32_t page[NCH], line[NCH];  // of the next tile's rows: scalars when `aligned`
@@ -540,8 +553,8 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             for (int i = 0; i < NCH; ++i) {
                 const uint32_t pg = __builtin_amdgcn_readfirstlane(min(page[i], p.b.npages - 1)), ln = __builtin_amdgcn_readfirstlane(line[i]);
                 const uint64_t at = (uint64_t)pg * (uint32_t)p.k_sp + ln * (uint32_t)p.k_sr;
-                kreg[i] = ld128(kh + at + off);
-                vreg[i] = ld128(vh + at + off);
+                kreg[i] = live ? ld128(kh + at + off) : u32x4{0, 0, 0, 0};
+                vreg[i] = live ? ld128(vh + at + off) : u32x4{0, 0, 0, 0};
             }
         } else {
 #pragma unroll
@@ -552,8 +565,8 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
                     const uint32_t key = t * BN + RS * i;
                     if (key < it.s.len) ln += min(cr, it.s.len - 1 - key);
                 }
-                kreg[i] = ld128(kb + (int64_t)pg * p.k_sp + (int64_t)ln * p.k_sr);
-                vreg[i] = ld128(vb + (int64_t)pg * p.v_sp + (int64_t)ln * p.v_sr);
+                kreg[i] = live ? ld128(kb + (int64_t)pg * p.k_sp + (int64_t)ln * p.k_sr) : u32x4{0, 0, 0, 0};
+                vreg[i] = live ? ld128(vb + (int64_t)pg * p.v_sp + (int64_t)ln * p.v_sr) : u32x4{0, 0, 0, 0};
             }
         }
     };
@@ -694,7 +707,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
     uint32_t bad = 0;
 #pragma unroll
     for (int w = 0; w < W; ++w) bad |= lds.bad[w];
-    if (bad) return paged_exactly<DH, ROWS>(p, it, first * BN, last * BN, W);
+    if (bad) return paged_exactly<DH, ROWS, PAD>(p, it, first * BN, last * BN, W);
     const float total = l + __shfl_xor(l, 32, WAVE);
     if (wrow + n32 >= it.nrows) return;
     // o[d][4 q + r]: column 32 d + 8 q + 4 h + r of the lane's query
@@ -721,7 +734,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 #pragma unroll
             for (int r = 0; r < 8; ++r) y.e[r] = f2e(o[d][4 * q + r] * inv);
             const uint32_t s0 = __shfl_xor(h ? y.u[0] : y.u[2], 32, WAVE), s1 = __shfl_xor(h ? y.u[1] : y.u[3], 32, WAVE);
-            st128(dst + 64 * d + 16 * q, h ? u32x4{s0, s1, y.u[2], y.u[3]} : u32x4{y.u[0], y.u[1], s0, s1});
+            if (!PAD || 32 * d + 8 * (q + h) < p.dh) st128(dst + 64 * d + 16 * q, h ? u32x4{s0, s1, y.u[2], y.u[3]} : u32x4{y.u[0], y.u[1], s0, s1});
         }
 }
 
@@ -729,7 +742,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 //
 // The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
 // way at a time, and the ranges are folded in one pass with a running maximum.
-template <int DH, int ROWS>
+template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
     constexpr int TPR = DH / 4, RPP = 256 / TPR;  // threads per row, rows per pass
     const uint32_t slot = blockIdx.x, col = 4 * (threadIdx.x % TPR);
@@ -738,7 +751,7 @@ __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
     // the grid allows for: what lies there must not lead outside the workspace or o.
     if (slot >= *reinterpret_cast<const uint32_t *>(p.work) || d.pieces < 2 || d.pieces > p.slots || d.piece >= d.pieces || d.kvh >= p.nkvh || d.nrows > ROWS) return;
     const uint64_t before = (uint64_t)d.piece * p.nkvh, behind = (uint64_t)(d.pieces - 1 - d.piece) * p.nkvh;
-    if (before > slot || slot + behind >= p.slots) return;
+    if (before > slot || slot + behind >= p.slots || (PAD && col >= p.dh)) return;
     const uint32_t slot0 = slot - (uint32_t)before;
     const size_t step = (size_t)p.nkvh * ROWS;
     for (uint32_t r = d.piece * RPP + threadIdx.x / TPR; r < d.nrows; r += d.pieces * RPP) {
@@ -784,14 +797,15 @@ __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
     }
 }
 
-template <int DH>
+// PAD: a head dimension of fewer columns than DH, a multiple of 8; the others are zero and not stored
+template <int DH, bool PAD>
 __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
     __shared__ __attribute__((aligned(16))) FewLds<DH> lds;
     PagedItem it;
-    if (paged_item<16, 4>(p, it)) paged_few<DH, 16>(p, it, lds);
+    if (paged_item<16, 4>(p, it)) paged_few<DH, 16, PAD>(p, it, lds);
 }
 // W waves of 32 rows: 4, two workgroups to a CU, or 8, one
-template <int DH, int W>
+template <int DH, int W, bool PAD>
 __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     __shared__ __attribute__((aligned(16))) union {
         FewLds<DH> few;
@@ -800,17 +814,20 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     PagedItem it;
     if (!paged_item<32 * W, W>(p, it)) return;
     if (it.s.n * p.group.d <= FEW) {
-        if (threadIdx.x < 4 * WAVE) paged_few<DH, 32 * W>(p, it, lds.few);  // (waves that have ended are not waited for)
-    } else paged_many<DH, W>(p, it, lds.many);
+        if (threadIdx.x < 4 * WAVE) paged_few<DH, 32 * W, PAD>(p, it, lds.few);  // (waves that have ended are not waited for)
+    } else paged_many<DH, W, PAD>(p, it, lds.many);
 }
 
-#define ATTN_PAGED(DH)                                                                                                                        \
-    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_few_d##DH)(AttnPagedParams p) { attn_paged_few<DH>(p); }       \
-    extern "C" __global__ void __launch_bounds__(256, 2) GEMM_KERNEL(attn_paged_many_d##DH)(AttnPagedParams p) { attn_paged_many<DH, 4>(p); }  \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 16>(p); } \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_d##DH)(AttnPagedParams p) { attn_paged_join<DH, 128>(p); }
-ATTN_PAGED(64)
-ATTN_PAGED(128)
+#define ATTN_PAGED(name, DH, PAD, PER_CU)                                                                                                                 \
+    extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_few_##name)(AttnPagedParams p) { attn_paged_few<DH, PAD>(p); }        \
+    extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_many_##name)(AttnPagedParams p) { attn_paged_many<DH, 4, PAD>(p); }   \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_##name)(AttnPagedParams p) { attn_paged_join<DH, 16, PAD>(p); }      \
+    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_##name)(AttnPagedParams p) { attn_paged_join<DH, 128, PAD>(p); }
+ATTN_PAGED(d64, 64, false, 2)
+ATTN_PAGED(d128, 128, false, 2)
+ATTN_PAGED(d64_pad, 64, true, 2)
+ATTN_PAGED(d128_pad, 128, true, 2)
+ATTN_PAGED(d256_pad, 256, true, 1)
 // (dh 64 gains nothing by tiles of 256: 8192 tokens, 32 heads over 8, 391 against 363 us)
-extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8>(p); }
-extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256>(p); }
+extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8, false>(p); }
+extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256, false>(p); }

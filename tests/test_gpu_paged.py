@@ -843,3 +843,38 @@ def test_attention_paged_sizes_between_the_kernels(gpu, stream, lens, nh, nkvh, 
 def test_qk_norm_rope_two_four_and_eight_tokens_per_workgroup(gpu, stream, nt, nh, nkh, dh):
     check_norm(gpu, stream, np.random.default_rng(42), nt, nh, nkh, dh, "f16", "f32", 10000.0)
     check_norm(gpu, stream, np.random.default_rng(43), nt, nh, nkh, dh, "bf16", "bf16", 0.0)
+
+
+@pytest.mark.parametrize("tile", ["0", "1"])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("dh", [8, 24, 56, 72, 80, 96, 120, 136, 192, 256])
+def test_attention_paged_head_dimensions_between(gpu, stream, monkeypatch, dh, kind, tile):
+    """Multiples of 8 that the matrix kernels fill up with zeros; NaN next to every row of the caches."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    for mask in (1, 0):
+        b = Batch(gpu, np.random.default_rng(44), kind, 4, 2, dh, 24, [(40, 90), (1, 600), (9, 9), (3, 2), (130, 200)], pad=1, head_gap=8)
+        want, tol = b.expected(mask)
+        check(attend(gpu, stream, b, mask), want, tol)
+
+
+@pytest.mark.parametrize("tile", ["0", "1"])
+@pytest.mark.parametrize("form", ["token_major", "odd_gap", "fused_qkv", "o_over_q", "unlike_caches", "descending"])
+@pytest.mark.parametrize("dh", [40, 96, 256])
+def test_attention_paged_views_of_other_head_dimensions(gpu, stream, monkeypatch, form, dh, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged_views(gpu, stream, form, (4, 2, dh, 16, [(50, 90), (1, 40), (3, 3)]))
+
+
+@pytest.mark.parametrize("tile", ["0", "1"])
+@pytest.mark.parametrize("kind,value", [("f16", np.nan), ("bf16", np.inf)])
+@pytest.mark.parametrize("dh", [96, 200])
+def test_attention_paged_what_is_masked_does_not_matter_for_other_heads(gpu, stream, monkeypatch, tile, kind, value, dh):
+    test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, tile, kind, value, dh)
+
+
+@pytest.mark.parametrize("dh", [36, 100, 250, 264, 512])
+def test_attention_paged_head_dimensions_of_no_matrix_kernel(gpu, stream, dh):
+    for kind in ("f16", "bf16", "f32"):
+        b = Batch(gpu, np.random.default_rng(45), kind, 4, 2, dh, 24, [(7, 90), (1, 200), (9, 9), (3, 2)], pad=1, head_gap=4)
+        want, tol = b.expected(1)
+        check(attend(gpu, stream, b, 1), want, tol)
