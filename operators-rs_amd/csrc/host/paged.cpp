@@ -127,16 +127,17 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 // ============================================================== attention_paged ===
 
 struct ophip_attention_paged : OpBase {
-    hipFunction_t any[3];
+    hipFunction_t any[3][4][2];  // [type][dh up to 64, 128, 256, 512][4 / 16 waves]
     // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64, 128, below 64, below 128, up to 256]; 256 rows for dh 128 only
     hipFunction_t rows[2][3][5], join[2][3][5];
     // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2
     // one size of tile (2: 1 where dh is 64)
     int slots = 0, tile = -1;
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
-        any[0] = d->kernel("attention_paged_any", "attn_paged_any_f16");
-        any[1] = d->kernel("attention_paged_any", "attn_paged_any_bf16");
-        any[2] = d->kernel("attention_paged_any", "attn_paged_any_f32");
+        static const char *const tag[3] = {"f16", "bf16", "f32"};
+        for (int t = 0; t < 3; ++t)
+            for (int n = 0; n < 4; ++n)
+                for (int w = 0; w < 2; ++w) any[t][n][w] = d->kernel("attention_paged_any", (std::string("attn_paged_any_") + tag[t] + "_n" + std::to_string(1 << n) + (w ? "_w16" : "")).c_str());
         for (int e = 0; e < 2; ++e)
             for (int r = 0; r < 3; ++r)
                 for (int h = 0; h < 5; ++h) {
@@ -207,11 +208,12 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
     const size_t steps = (m.cols * m.page + 31) / 32;
     const size_t most = std::max<size_t>(1, steps / 4);  // (a key range has four steps of 32 keys at least)
-    // Key ranges for all tiles together: as many as workgroups of 128 or 256 rows run at a time (two or one per CU; 511 tokens over
+    // Key ranges for all tiles together: as many as workgroups of 128 or 256 rows run at a time (two or one per CU, one for heads
+    // above 128; 511 tokens over
     // 32511 keys, 32 heads over 8, on tiles of 128: 420 us with half as many, 321, 338 with twice as many), and four per CU
     // for 16 rows, where a range costs little and the rates of memory even out (50 decode steps over 165008 keys: 134 us
     // with 512, 122 with 1024, 124 with 1536).
-    const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 ? 2 : 1) * cus;
+    const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 && dh <= 128 ? 2 : 1) * cus;
     a.grid = units;
     if (most > 1) {
         a.slots = std::min((4 * want + 2) / 3, units * most);
@@ -271,7 +273,9 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         return;
     }
     op->dev->make_current();
-    launch(op->any[type_index(m.dt)], Dim3{(unsigned)nt, (unsigned)nh}, Dim3{256}, 0, stream_of(qa), p);
+    // sixteen waves to a row where there are no more than two rows to a CU
+    const int n = dh <= 64 ? 0 : dh <= 128 ? 1 : dh <= 256 ? 2 : 3, w = nt * nh <= 2 * (size_t)op->dev->props.multiProcessorCount;
+    launch(op->any[type_index(m.dt)][n][w], Dim3{(unsigned)nt, (unsigned)nh}, Dim3{w ? 1024u : 256u}, 0, stream_of(qa), p);
 }
 
 }  // namespace

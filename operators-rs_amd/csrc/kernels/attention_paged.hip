@@ -68,13 +68,13 @@ __device__ __forceinline__ uint32_t paged_pieces(const AttnPagedParams &p, const
 }
 // Ranges per unit of weight.  `work`: tiles times weight of all sequences.  As many as there are slots (three quarters: a count
 // rounded to two or more is at most four thirds of what it was) for long batches, but beyond one per CU only while each has
-// 24 steps of its own, or 8 of a tile that weighs twice: the plan, the first loads and the join cost as much as several
+// 24 steps of its own (12 of heads above 128), or 8 of a tile that weighs twice: the plan, the first loads and the join cost as much as several
 // steps (31 decode steps over 57 MB in 1024 / 512 / 256 ranges: 27.9 / 19.4 / 17.5 us).
 template <int ROWS>
 __device__ __forceinline__ float paged_per_step(const AttnPagedParams &p, float work) {
     if (!(work > 0.f)) return 0.f;
     const float all = work * (float)p.nkvh;
-    return fminf(0.74999f * (float)p.slots, fmaxf((float)p.cus, all * (1.f / (ROWS == FEW ? 24.f : 16.f)))) / all;
+    return fminf(0.74999f * (float)p.slots, fmaxf((float)p.cus, all * (1.f / (ROWS == FEW && p.dh <= 128 ? 24.f : ROWS == FEW ? 12.f : 16.f)))) / all;
 }
 
 // What workgroup blockIdx.x does; false: nothing.  Every thread calls it and gets the same.

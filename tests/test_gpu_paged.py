@@ -878,3 +878,17 @@ def test_attention_paged_head_dimensions_of_no_matrix_kernel(gpu, stream, dh):
         b = Batch(gpu, np.random.default_rng(45), kind, 4, 2, dh, 24, [(7, 90), (1, 200), (9, 9), (3, 2)], pad=1, head_gap=4)
         want, tol = b.expected(1)
         check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("kind,dh", [("f32", 64), ("f32", 100), ("f32", 250), ("f32", 512), ("bf16", 36), ("f16", 500)])
+def test_attention_paged_more_rows_of_no_matrix_kernel(gpu, stream, kind, dh):
+    """Beyond two rows to a CU, each has four waves."""
+    for mask in (1, 0):
+        b = Batch(gpu, np.random.default_rng(46), kind, 8, 2, dh, 7, [(80, 95), (1, 40), (3, 2)], pad=2, head_gap=4)
+        want, tol = b.expected(mask)
+        check(attend(gpu, stream, b, mask), want, tol)
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_attention_paged_what_is_masked_does_not_matter_in_f32(gpu, stream, monkeypatch, value):
+    test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, "0", "f32", value, 100)
