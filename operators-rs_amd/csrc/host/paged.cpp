@@ -208,11 +208,11 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
     const size_t steps = (m.cols * m.page + 31) / 32;
     const size_t most = std::max<size_t>(1, steps / 4);  // (a key range has four steps of 32 keys at least)
-    // Key ranges for all tiles together: as many as workgroups of 128 or 256 rows run at a time (two or one per CU, one for heads
-    // above 128; 511 tokens over
-    // 32511 keys, 32 heads over 8, on tiles of 128: 420 us with half as many, 321, 338 with twice as many), and four per CU
-    // for 16 rows, where a range costs little and the rates of memory even out (50 decode steps over 165008 keys: 134 us
-    // with 512, 122 with 1024, 124 with 1536).
+    // Key ranges for all tiles together: as many as workgroups of 128 or 256 rows run at a time (two or one per CU, one for
+    // heads above 128; 511 tokens over 32511 keys, 32 heads over 8, on tiles of 128: 420 us with half as many, 321, 338 with twice
+    // as many), and four per CU for 16 rows, where a range costs little and the rates of memory even out (50 decode steps
+    // over 165008 keys: 134 us with 512, 122 with 1024, 124 with 1536).  The device makes fewer of them for short batches
+    // (paged_per_step).
     const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 && dh <= 128 ? 2 : 1) * cus;
     a.grid = units;
     if (most > 1) {

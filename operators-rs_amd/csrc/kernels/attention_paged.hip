@@ -1,20 +1,23 @@
 // attention over a paged cache on the matrix cores: o = softmax(scale q . k^T) . v for a packed batch of sequences of
-// unlike lengths, f16 / bf16, dh 64 and 128.
+// unlike lengths, f16 / bf16, head dimensions of a multiple of 8 up to 256 (kernels for 64, 128 and 256 columns).
 //
 // Work units.  The query rows of one kv head and sequence are its new tokens times the `group` query heads that share
 // the kv head, row = token * group + head-in-group.  A sequence of up to 16 rows (a decode step) is one tile that
-// paged_few works on: the caches are all the traffic.  One of more rows (prompts, chunks) is cut into tiles of 128 rows for
-// paged_many: the products are the work.  So keys and values are read once per tile whatever the group, and a short
-// group fills the rows with further tokens.  Two kernels: attn_paged_few, on tiles of 16 rows only, for batches that are
-// nearly all decode steps, and attn_paged_many, which has both inside and gives each sequence its own (25 sequences
-// over 56185 keys, one of them a chunk of 333 tokens, dh 64: 36 us with all of them on tiles of 128 rows, BOTH with both).
+// paged_few works on: the caches are all the traffic.  One of more rows (prompts, chunks) is cut into tiles of 128 or 256 rows
+// for paged_many: the products are the work.  So keys and values are read once per tile whatever the group, and a short
+// group fills the rows with further tokens.  Three kernels: attn_paged_few, on tiles of 16 rows only, for batches that are
+// nearly all decode steps and for little work; attn_paged_many, which has both inside and gives each sequence its own (24 decode
+// steps and a chunk of 333 tokens over 56185 keys in all, dh 64: 35 us; on tiles of 16 rows alone 59); attn_paged_wide, the same
+// on tiles of 256 rows, for long sequences.  The host chooses by sizes (attention_paged_plan).
 //
 // Plan.  The host knows the number of tokens and sequences, not the lengths, and must not wait for them; so every
-// workgroup works its own unit out from the lengths on the device (paged_item: a prefix sum over the sequences).  The tiles
-// of a sequence with more keys than 1 / slots of all tiles' keys are cut into that many more key ranges, one workgroup
+// workgroup works its own unit out from the lengths on the device (paged_item: a prefix sum over the sequences, 2.5 to 3.5 us).
+// The tiles of a sequence with more keys than 1 / slots of all tiles' keys are cut into that many more key ranges, one workgroup
 // each, so that a launch has about `slots` equal pieces of work whatever the mix of lengths.  Ranges of a cut tile leave
 // their maximum, sum and output in the workspace and attn_paged_join merges them in a fixed order: results do not
-// depend on which workgroup ends first.
+// depend on which workgroup ends first.  (Joining in the first launch, by the workgroup that finds all ranges of its tile
+// there, spares a launch of 3 us but makes every workgroup wait for its stores: a decode step over 2048 keys 12.1 us against
+// 11.3, 47 of them 127 against 118.)
 //
 // Compiled twice, like the other MFMA kernels (gemm_elem.h).
 #include "gemm_elem.h"
@@ -266,7 +269,9 @@ __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const Pa
 //   O^T = V^T . P^T, contraction slot 8 g + 4 c + i being key 16 c + 4 g + i.  A is then the values of those eight keys, of
 //   which the lane reads DH / 16 adjacent columns each and transposes them in registers.
 // The matrix cores are idle most of the time: 16 KB of keys and values take about 500 cycles of one wave, a CU's share of
-// the memory's rate delivers them in 1300.
+// the memory's rate delivers them in 1300.  Memory bounds it: 50 decode steps over 165008 keys, 8 kv heads of 128, 676 MB,
+// 118 us, 5.75 TB/s (a pure read of that size with the non-temporal hint 6.46, a copy 4.89); below some 50 MB the latencies of the
+// launches, the plan and a range's first loads do (one step over 2047 keys, 8 MB: 11 us, of which 9 are the two launches).
 template <int CW>
 struct FewTile {  // 32 keys
     u32x4 k[2][CW / 2];
@@ -488,6 +493,12 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
 // query and half the tile's keys, so maxima, sums and factors are scalars of the lane; the probabilities are packed in
 // registers into B operands of O^T = V^T . P^T, whose A operands come from the row-major tile through the transposing
 // LDS read.  A wave without rows, or whose rows all end before a tile, only helps to load.
+// What bounds it is the matrix cores' rate together with the exponentials that their order leaves between the products: 8192
+// tokens, 32 heads over 8 of 128, causal, 0.55 Tflop kept: 565 us, 0.97 PF (a plain product of 8192^3 reaches 1.24) with eight
+// waves that share a tile's loads, 602 with four; 511 tokens over 32511 keys 290 us, 0.93 PF (machines differ by a tenth).  In
+// the order that the compiler gives them, products, LDS reads and the second half's exponentials took 633 us where the one
+// below took 593; a raised priority of the wave around its products changed nothing.  Short prompts are bound by a unit's
+// fixed time, some 6 us: 7 prompts of 104 to 546 tokens, 32 heads of 128: 30 us.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int DH>
@@ -616,7 +627,6 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
         }
         if ((int32_t)(t * BN) < lim_last) {
             const elem *kt = lds.k[buf], *vt = lds.v[buf];
-            __builtin_amdgcn_s_setprio(1);
             // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
             f32x16 sacc[2];
 #pragma unroll
@@ -637,7 +647,6 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            __builtin_amdgcn_s_setprio(0);
             if ((int32_t)(t * BN + BN) > lim_first) {
 #pragma unroll
                 for (int b = 0; b < 2; ++b)
@@ -686,7 +695,6 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 #pragma unroll
                 for (int e = 0; e < 16; ++e) power(0, e);
                 __builtin_amdgcn_sched_barrier(0);
-                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     o[i % DB] = mfma_32x32x16(a[i].hv, pb[i / DB].h, o[i % DB]);
@@ -698,7 +706,6 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
                 }
             }
         }
-        __builtin_amdgcn_s_setprio(0);
         if (more) commit(buf ^ 1, t + 1);
         __syncthreads();
     }
@@ -740,7 +747,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 
 // ---- the ranges of a cut tile: o = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
 //
-// The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
+// (2.5 to 5 us, nearly all latency; 9 for the 256-row tiles of 511 tokens over 32511 keys, 44 MB.)  The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
 // way at a time, and the ranges are folded in one pass with a running maximum.
 template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
