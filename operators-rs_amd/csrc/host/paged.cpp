@@ -215,7 +215,14 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     // (paged_per_step).
     const size_t want = op && op->slots > 0 ? (size_t)op->slots : (a.tile == 0 ? 4 : a.tile == 1 && dh <= 128 ? 2 : 1) * cus;
     a.grid = units;
-    if (most > 1) {
+    // No ranges, and no second launch, where a tile takes its keys in less time than cutting and joining would cost: short ones, and
+    // longer ones where the tiles fill the machine as it is (615 tokens of 2 sequences, 64 heads over 4, up to 597 keys: 25.1 us
+    // against 37.1 with ranges; 4097 tokens of 17 sequences, 16 heads over 1, 923 keys: 35.6 against 41.1; on tiles of 16 rows,
+    // up to 384 keys: 8.4 against 10.0; past the bounds, a quarter of the machine and 1024 keys: 22.1 against 20.3, an
+    // eighth, on tiles of 16 rows: 15.9 against 14.8).
+    const size_t len = m.cols * m.page, have = m.nkvh * rows, fill = want * tile;
+    const bool whole = a.tile == 0 ? len <= 512 || (len <= 1024 && have >= fill / 8) : len <= 768 || (len <= 1024 && have >= fill / 4) || (len <= 2048 && have >= fill);
+    if (most > 1 && !whole) {
         a.slots = std::min((4 * want + 2) / 3, units * most);
         a.grid = std::min(units * most, units + (4 * want + 2) / 3);
         a.workspace = 64 + a.slots * (32 + tile * (dh + 2) * sizeof(float));

@@ -892,3 +892,11 @@ def test_attention_paged_more_rows_of_no_matrix_kernel(gpu, stream, kind, dh):
 @pytest.mark.parametrize("value", [np.nan, np.inf])
 def test_attention_paged_what_is_masked_does_not_matter_in_f32(gpu, stream, monkeypatch, value):
     test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, "0", "f32", value, 100)
+
+
+@pytest.mark.parametrize("tile,dh", [("0", 64), ("0", 96), ("1", 128), ("1", 200), ("2", 128)])
+@pytest.mark.parametrize("form", ["token_major", "fused_qkv", "o_over_q", "strided_batch", "descending"])
+def test_attention_paged_views_of_long_caches(gpu, stream, monkeypatch, form, tile, dh):
+    """Lengths at which ranges are cut, so that the join writes o."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    test_attention_paged_views(gpu, stream, form, (4, 2, dh, 32, [(20, 1500), (1, 2100), (3, 3), (5, 1200)]))
