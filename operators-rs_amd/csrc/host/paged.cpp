@@ -276,7 +276,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         const int e = m.dt == OPHIP_DT_BF16, h = plan.head;
         op->dev->make_current();
         launch(op->rows[e][plan.tile][h], Dim3{(unsigned)plan.grid}, Dim3{plan.tile == 2 ? 512u : 256u}, 0, stream_of(qa), p);
-        if (plan.slots) launch(op->join[e][plan.tile][h], Dim3{(unsigned)plan.slots}, Dim3{256}, 0, stream_of(qa), p);
+        if (plan.slots) launch(op->join[e][plan.tile][h], Dim3{(unsigned)plan.slots}, Dim3{plan.tile ? 512u : 256u}, 0, stream_of(qa), p);
         return;
     }
     op->dev->make_current();

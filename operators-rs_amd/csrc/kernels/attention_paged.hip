@@ -747,11 +747,13 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
 
 // ---- the ranges of a cut tile: o = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c
 //
-// (2.5 to 5 us, nearly all latency; 9 for the 256-row tiles of 511 tokens over 32511 keys, 44 MB.)  The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
-// way at a time, and the ranges are folded in one pass with a running maximum.
+// The rows of a tile are dealt out to the workgroups of its ranges, DH / 4 threads to a row; four ranges' loads are on their
+// way at a time, and the ranges are folded in one pass with a running maximum.  2.5 to 5 us, nearly all latency; 8 for the
+// 256-row tiles of 511 tokens over 32511 keys, 34 MB.  Large tiles have eight waves (of four, eight and sixteen: 298 / 296 /
+// 299 us for those tokens, 0.6 % between the first two over 250 drawn batches).
 template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
-    constexpr int TPR = DH / 4, RPP = 256 / TPR;  // threads per row, rows per pass
+    constexpr int TPR = DH / 4, RPP = (ROWS == FEW ? 256 : 512) / TPR;  // threads per row, rows per pass
     const uint32_t slot = blockIdx.x, col = 4 * (threadIdx.x % TPR);
     const PagedDesc d = paged_desc(p)[slot];
     // Slots behind the count hold no descriptor; nor do those of a batch whose sequences overlap, when it has more tiles than
@@ -829,7 +831,7 @@ __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_few_##name)(AttnPagedParams p) { attn_paged_few<DH, PAD>(p); }        \
     extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_many_##name)(AttnPagedParams p) { attn_paged_many<DH, 4, PAD>(p); }   \
     extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_##name)(AttnPagedParams p) { attn_paged_join<DH, 16, PAD>(p); }      \
-    extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_many_##name)(AttnPagedParams p) { attn_paged_join<DH, 128, PAD>(p); }
+    extern "C" __global__ void __launch_bounds__(512) GEMM_KERNEL(attn_paged_join_many_##name)(AttnPagedParams p) { attn_paged_join<DH, 128, PAD>(p); }
 ATTN_PAGED(d64, 64, false, 2)
 ATTN_PAGED(d128, 128, false, 2)
 ATTN_PAGED(d64_pad, 64, true, 2)
@@ -837,4 +839,4 @@ ATTN_PAGED(d128_pad, 128, true, 2)
 ATTN_PAGED(d256_pad, 256, true, 1)
 // (dh 64 gains nothing by tiles of 256: 8192 tokens, 32 heads over 8, 391 against 363 us)
 extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8, false>(p); }
-extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256, false>(p); }
+extern "C" __global__ void __launch_bounds__(512) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256, false>(p); }
