@@ -900,3 +900,25 @@ def test_attention_paged_views_of_long_caches(gpu, stream, monkeypatch, form, ti
     """Lengths at which ranges are cut, so that the join writes o."""
     monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
     test_attention_paged_views(gpu, stream, form, (4, 2, dh, 32, [(20, 1500), (1, 2100), (3, 3), (5, 1200)]))
+
+
+@pytest.mark.parametrize("tile", ["0", "1", "2"])
+def test_attention_paged_tokens_in_front_of_the_first_sequence(gpu, stream, monkeypatch, tile):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(47), "f16", 4, 2, 128, 16, [(30, 70), (1, 1400), (40, 55)], pad=3)
+    b.lens[0], b.start[0] = (23, 70), 7  # seven tokens of no sequence, then the first's 23
+    b.q_start = Buffer(gpu, b.start)
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("nh,nkvh", [(128, 1), (96, 2), (64, 64), (130, 2)])
+def test_attention_paged_wide_groups_and_many_heads(gpu, stream, nh, nkvh):
+    b = Batch(gpu, np.random.default_rng(48), "bf16", nh, nkvh, 64, 16, [(1, 90), (2, 33), (3, 3)], pad=1)
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("nt,nh,nkh,dh", [(600, 6, 2, 128), (300, 2, 2, 64), (2100, 3, 1, 64)])
+def test_qk_norm_rope_in_place_with_several_tokens_per_workgroup(gpu, stream, nt, nh, nkh, dh):
+    check_norm(gpu, stream, np.random.default_rng(49), nt, nh, nkh, dh, "f16", "f32", 10000.0, "in_place")
