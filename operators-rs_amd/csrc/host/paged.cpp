@@ -128,10 +128,11 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 
 struct ophip_attention_paged : OpBase {
     hipFunction_t any[3][4][2];  // [type][dh up to 64, 128, 256, 512][4 / 16 waves]
-    // [f16 / bf16][tiles of 16 / 128 / 256 rows][dh 64, 128, below 64, below 128, up to 256]; 256 rows for dh 128 only
-    hipFunction_t rows[2][3][5], join[2][3][5];
-    // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2
-    // one size of tile (2: 1 where dh is 64)
+    // [f16 / bf16][tiles of 16 / 128 / 256 / 128 rows for two groups][dh 64, 128, below 64, below 128, up to 256]; 256 rows for dh 128
+    // only, two groups for 64 and 128
+    hipFunction_t rows[2][4][5], join[2][4][5];
+    // read once, here (tests, sweeps): OPHIP_ATTN_PAGED_SLOTS=<n> key ranges to cut a launch into, OPHIP_ATTN_PAGED_TILE=0|1|2|3
+    // one kind of tile (1 where there is no other for the head dimension)
     int slots = 0, tile = -1;
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
         static const char *const tag[3] = {"f16", "bf16", "f32"};
@@ -139,14 +140,15 @@ struct ophip_attention_paged : OpBase {
             for (int n = 0; n < 4; ++n)
                 for (int w = 0; w < 2; ++w) any[t][n][w] = d->kernel("attention_paged_any", (std::string("attn_paged_any_") + tag[t] + "_n" + std::to_string(1 << n) + (w ? "_w16" : "")).c_str());
         for (int e = 0; e < 2; ++e)
-            for (int r = 0; r < 3; ++r)
+            for (int r = 0; r < 4; ++r)
                 for (int h = 0; h < 5; ++h) {
-                    if (r == 2 && h != 1) continue;
+                    if ((r == 2 && h != 1) || (r == 3 && h > 1)) continue;
                     static const char *const head[5] = {"d64", "d128", "d64_pad", "d128_pad", "d256_pad"};
                     const char *mod = e ? "attention_paged_bf16" : "attention_paged";
-                    const std::string tail = std::string(r == 0 ? "few_" : r == 1 ? "many_" : "wide_") + head[h] + (e ? "_bf16" : "");
-                    rows[e][r][h] = d->kernel(mod, ("attn_paged_" + tail).c_str());
-                    join[e][r][h] = d->kernel(mod, ("attn_paged_join_" + tail).c_str());
+                    const std::string tail = std::string(head[h]) + (e ? "_bf16" : "");
+                    static const char *const of[4] = {"few_", "many_", "wide_", "pair_"};
+                    rows[e][r][h] = d->kernel(mod, ("attn_paged_" + (of[r] + tail)).c_str());
+                    join[e][r][h] = d->kernel(mod, ("attn_paged_join_" + (of[r == 3 ? 1 : r] + tail)).c_str());
                 }
         if (const char *e = std::getenv("OPHIP_ATTN_PAGED_SLOTS")) slots = std::atoi(e);
         if (const char *e = std::getenv("OPHIP_ATTN_PAGED_TILE")) tile = std::atoi(e);
@@ -178,7 +180,7 @@ AttnPagedMeta attention_paged_meta(const ophip_attention_paged_args &a) {
 // How the matrix kernels take a call (attention_paged.hip), from its sizes alone.
 struct AttnPagedPlan {
     bool matrix;                    // they serve these types and sizes
-    int tile, head;                 // tiles of 16, 128 or 256 rows: 0, 1, 2; of the kernels' head dimensions
+    int tile, head;                 // tiles of 16, 128 or 256 rows, or of 128 for two groups of waves: 0, 1, 2, 3; of the kernels' head dimensions
     size_t grid, slots;  // workgroups; key ranges the workspace holds (0: no tile can be cut)
     size_t workspace;
 };
@@ -200,10 +202,18 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     // 32 heads over 8: 558 against 585 us, 511 tokens over 32511 keys 299 against 318; shorter than the bound, 7 prompts of up
     // to 546 tokens 36.8 against 32.6; dh 64 never gains by them).
     const size_t group = m.nh / m.nkvh, rows = m.nt * group, products = m.nkvh * rows * (m.page * m.cols);  // (below 2^61)
+    // Tiles of 128 that two groups of waves share, half of the keys each, where there is about one for each CU or fewer and no
+    // ranges are cut (70 batches of up to 768 keys, up to 1024 with three quarters of the CUs, 6 to 17 % faster, the worst 5 %
+    // slower).  With more tiles the second workgroup of a CU serves better than the second group (some 450 rows to a
+    // sequence, 32 kv heads of 64, up to 600 keys: 47 against 28 us), with more keys ranges do, as often as not (133 batches
+    // of up to 4096 keys between 0.74 and 1.38 times as long).
+    const size_t len = m.cols * m.page, tiles128 = m.nkvh * (rows + std::min(m.nseq, m.nt) * 127);  // times 128, at the most
     if ((products <= cus << 14 && m.nkvh * rows <= cus << 5) || (group <= 16 && m.nt <= 2 * m.nseq)) a.tile = 0;
-    else a.tile = m.dh == 128 && rows >= 1024 * m.nseq && products >= cus << 20 ? 2 : 1;
-    if (op && op->tile >= 0 && op->tile <= 2) a.tile = m.dh == 128 ? op->tile : std::min(op->tile, 1);
-    const size_t tile = a.tile == 0 ? 16 : a.tile == 1 ? 128 : 256;
+    else if (m.dh == 128 && rows >= 1024 * m.nseq && products >= cus << 20) a.tile = 2;
+    else a.tile = a.head <= 1 && tiles128 <= 154 * cus && rows >= 64 * m.nseq && len <= (tiles128 >= 96 * cus ? 1024u : 768u) ? 3 : 1;
+    if (op && op->tile >= 0 && op->tile <= 3) a.tile = op->tile;
+    if ((a.tile == 2 && m.dh != 128) || (a.tile == 3 && a.head > 1)) a.tile = 1;
+    const size_t tile = a.tile == 0 ? 16 : a.tile == 2 ? 256 : 128;
     // the most tiles there can be, whatever the lengths: each sequence that has a token may have one that is not full
     const size_t units = m.nkvh * ((rows + std::min(m.nseq, m.nt) * (tile - 1)) / tile);
     const size_t steps = (m.cols * m.page + 31) / 32;
@@ -220,7 +230,7 @@ AttnPagedPlan attention_paged_plan(const ophip_attention_paged *op, const AttnPa
     // against 37.1 with ranges; 4097 tokens of 17 sequences, 16 heads over 1, 923 keys: 35.6 against 41.1; on tiles of 16 rows,
     // up to 384 keys: 8.4 against 10.0; past the bounds, a quarter of the machine and 1024 keys: 22.1 against 20.3, an
     // eighth, on tiles of 16 rows: 15.9 against 14.8).
-    const size_t len = m.cols * m.page, have = m.nkvh * rows, fill = want * tile;
+    const size_t have = m.nkvh * rows, fill = want * tile;
     const bool whole = a.tile == 0 ? len <= 512 || (len <= 1024 && have >= fill / 8) : len <= 768 || (len <= 1024 && have >= fill / 4) || (len <= 2048 && have >= fill);
     if (most > 1 && !whole) {
         a.slots = std::min((4 * want + 2) / 3, units * most);
@@ -275,7 +285,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
                    p.b.t_col >= 0 && p.b.t_col < far / (ptrdiff_t)p.b.cols;
         const int e = m.dt == OPHIP_DT_BF16, h = plan.head;
         op->dev->make_current();
-        launch(op->rows[e][plan.tile][h], Dim3{(unsigned)plan.grid}, Dim3{plan.tile == 2 ? 512u : 256u}, 0, stream_of(qa), p);
+        launch(op->rows[e][plan.tile][h], Dim3{(unsigned)plan.grid}, Dim3{plan.tile >= 2 ? 512u : 256u}, 0, stream_of(qa), p);
         if (plan.slots) launch(op->join[e][plan.tile][h], Dim3{(unsigned)plan.slots}, Dim3{plan.tile ? 512u : 256u}, 0, stream_of(qa), p);
         return;
     }

@@ -5,10 +5,11 @@
 // the kv head, row = token * group + head-in-group.  A sequence of up to 16 rows (a decode step) is one tile that
 // paged_few works on: the caches are all the traffic.  One of more rows (prompts, chunks) is cut into tiles of 128 or 256 rows
 // for paged_many: the products are the work.  So keys and values are read once per tile whatever the group, and a short
-// group fills the rows with further tokens.  Three kernels: attn_paged_few, on tiles of 16 rows only, for batches that are
+// group fills the rows with further tokens.  Four kernels: attn_paged_few, on tiles of 16 rows only, for batches that are
 // nearly all decode steps and for little work; attn_paged_many, which has both inside and gives each sequence its own (24 decode
 // steps and a chunk of 333 tokens over 56185 keys in all, dh 64: 35 us; on tiles of 16 rows alone 59); attn_paged_wide, the same
-// on tiles of 256 rows, for long sequences.  The host chooses by sizes (attention_paged_plan).
+// on tiles of 256 rows, for long sequences; attn_paged_pair, the same on tiles of 128 rows whose keys two groups of waves
+// take in turn, for so few tiles that a CU has one at the most.  The host chooses by sizes (attention_paged_plan).
 //
 // Plan.  The host knows the number of tokens and sequences, not the lengths, and must not wait for them; so every
 // workgroup works its own unit out from the lengths on the device (paged_item: a prefix sum over the sequences, 2.5 to 3.5 us).
@@ -509,12 +510,15 @@ struct ManyLds {
     uint32_t bad[8];  // by wave: values that are not finite, in a tile that some row keeps in part
 };
 
-template <int DH, int W, bool PAD>
-__device__ __forceinline__ void paged_many(const AttnPagedParams &p, const PagedItem &it, ManyLds<DH> &lds) {
+// G groups of W waves share the rows; each takes every G-th tile of keys into LDS of its own, and the second hands its maxima,
+// sums and outputs to the first through LDS.
+template <int DH, int W, int G, bool PAD>
+__device__ __forceinline__ void paged_many(const AttnPagedParams &p, const PagedItem &it, ManyLds<DH> (&both)[G]) {
     constexpr int BN = ManyLds<DH>::BN, KP = ManyLds<DH>::KP, VP = ManyLds<DH>::VP;
     constexpr int CPR = DH / 8, ROWS = 32 * W, NCH = BN * CPR / (W * WAVE), RS = W * WAVE / CPR;  // 16-byte chunks per row, per thread; rows between a thread's chunks
     constexpr int DS = DH / 16, DB = DH / 32;
-    const uint32_t tid = threadIdx.x, wave = tid / WAVE, lane = tid % WAVE;
+    const uint32_t group = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / (W * WAVE)), tid = threadIdx.x - group * (W * WAVE), wave = tid / WAVE, lane = tid % WAVE;
+    ManyLds<DH> &lds = both[group];
     const uint32_t n32 = lane % 32, h = lane / 32, s16 = lane % 16, b16 = (lane / 16) % 2;
     const uint32_t wrow = wave * 32, at = min(wrow + n32, it.nrows - 1);
     const uint32_t row = it.row0 + at, token = fastdiv(row, p.group), head = it.kvh * p.group.d + (row - token * p.group.d);
@@ -609,23 +613,24 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
     float m = -INFINITY, l = 0.f;
     const float scale2 = p.scale * PA_LOG2E;  // (positive: maxima commute with it)
 
-    if (first < last) {
-        look_up(first);
-        fetch(first);
-        commit(0, first);
-        if (first + 1 < last) look_up(first + 1);
+    if (first + group < last) {
+        look_up(first + group);
+        fetch(first + group);
+        commit(0, first + group);
+        if (first + group + G < last) look_up(first + group + G);
     }
 #pragma unroll
     for (int d = 0; d < DS; ++d) OPHIP_ARRIVED(qf[d].u);
     __syncthreads();
-    for (uint32_t t = first; t < last; ++t) {
-        const int buf = (t - first) & 1;
-        const bool more = t + 1 < last;
+    for (uint32_t t0 = first; t0 < last; t0 += G) {
+        const uint32_t t = t0 + group;
+        const int buf = (t0 - first) / G & 1;
+        const bool more = t + G < last;
         if (more) {
-            fetch(t + 1);
-            look_up(t + 2);
+            fetch(t + G);
+            look_up(t + 2 * G);
         }
-        if ((int32_t)(t * BN) < lim_last) {
+        if ((int32_t)(t * BN) < lim_last && (G == 1 || t < last)) {
             const elem *kt = lds.k[buf], *vt = lds.v[buf];
             // sacc[b][e]: key 32 b + 8 (e / 4) + 4 h + e % 4 of the tile, query n32
             f32x16 sacc[2];
@@ -706,16 +711,44 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
                 }
             }
         }
-        if (more) commit(buf ^ 1, t + 1);
+        if (more) commit(buf ^ 1, t + G);
         __syncthreads();
     }
     if (lane == 0) lds.bad[wave] = spoiled;
     __syncthreads();
     uint32_t bad = 0;
 #pragma unroll
-    for (int w = 0; w < W; ++w) bad |= lds.bad[w];
-    if (bad) return paged_exactly<DH, ROWS, PAD>(p, it, first * BN, last * BN, W);
-    const float total = l + __shfl_xor(l, 32, WAVE);
+    for (int w = 0; w < W * G; ++w) bad |= both[w / W].bad[w % W];
+    if (bad) return paged_exactly<DH, ROWS, PAD>(p, it, first * BN, last * BN, W * G);
+    float total = l + __shfl_xor(l, 32, WAVE);
+    if constexpr (G == 2) {  // the second group's results, where its tiles were
+        static_assert(sizeof(ManyLds<DH>) - sizeof lds.bad >= (size_t)W * WAVE * (DB * 16 + 2) * sizeof(float));
+        f32x4 *out = reinterpret_cast<f32x4 *>(both[1].k) + tid;
+        f32x2 *stats = reinterpret_cast<f32x2 *>(reinterpret_cast<f32x4 *>(both[1].k) + DB * 4 * W * WAVE) + tid;
+        __syncthreads();
+        if (group == 1) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) out[(4 * d + q) * W * WAVE] = f32x4{o[d][4 * q], o[d][4 * q + 1], o[d][4 * q + 2], o[d][4 * q + 3]};
+            *stats = f32x2{m, total};
+        }
+        __syncthreads();
+        if (group == 1) return;
+        const f32x2 other = *stats;
+        const float now = fmaxf(m, other[0]), ref = now == -INFINITY ? 0.f : now;
+        const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = __builtin_amdgcn_exp2f(other[0] - ref);
+        total = total * f0 + other[1] * f1;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 x = out[(4 * d + q) * W * WAVE];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[d][4 * q + r] = o[d][4 * q + r] * f0 + x[r] * f1;
+            }
+        m = now;
+    }
     if (wrow + n32 >= it.nrows) return;
     // o[d][4 q + r]: column 32 d + 8 q + 4 h + r of the lane's query
     if (it.pieces > 1) {
@@ -813,23 +846,23 @@ __device__ __forceinline__ void attn_paged_few(const AttnPagedParams &p) {
     PagedItem it;
     if (paged_item<16, 4>(p, it)) paged_few<DH, 16, PAD>(p, it, lds);
 }
-// W waves of 32 rows: 4, two workgroups to a CU, or 8, one
-template <int DH, int W, bool PAD>
+// G groups of W waves of 32 rows: 4, two workgroups to a CU, or 8 in one or two groups, one
+template <int DH, int W, int G, bool PAD>
 __device__ __forceinline__ void attn_paged_many(const AttnPagedParams &p) {
     __shared__ __attribute__((aligned(16))) union {
         FewLds<DH> few;
-        ManyLds<DH> many;
+        ManyLds<DH> many[G];
     } lds;
     PagedItem it;
-    if (!paged_item<32 * W, W>(p, it)) return;
+    if (!paged_item<32 * W, W * G>(p, it)) return;
     if (it.s.n * p.group.d <= FEW) {
         if (threadIdx.x < 4 * WAVE) paged_few<DH, 32 * W, PAD>(p, it, lds.few);  // (waves that have ended are not waited for)
-    } else paged_many<DH, W, PAD>(p, it, lds.many);
+    } else paged_many<DH, W, G, PAD>(p, it, lds.many);
 }
 
 #define ATTN_PAGED(name, DH, PAD, PER_CU)                                                                                                                 \
     extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_few_##name)(AttnPagedParams p) { attn_paged_few<DH, PAD>(p); }        \
-    extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_many_##name)(AttnPagedParams p) { attn_paged_many<DH, 4, PAD>(p); }   \
+    extern "C" __global__ void __launch_bounds__(256, PER_CU) GEMM_KERNEL(attn_paged_many_##name)(AttnPagedParams p) { attn_paged_many<DH, 4, 1, PAD>(p); }   \
     extern "C" __global__ void __launch_bounds__(256) GEMM_KERNEL(attn_paged_join_few_##name)(AttnPagedParams p) { attn_paged_join<DH, 16, PAD>(p); }      \
     extern "C" __global__ void __launch_bounds__(512) GEMM_KERNEL(attn_paged_join_many_##name)(AttnPagedParams p) { attn_paged_join<DH, 128, PAD>(p); }
 ATTN_PAGED(d64, 64, false, 2)
@@ -838,5 +871,7 @@ ATTN_PAGED(d64_pad, 64, true, 2)
 ATTN_PAGED(d128_pad, 128, true, 2)
 ATTN_PAGED(d256_pad, 256, true, 1)
 // (dh 64 gains nothing by tiles of 256: 8192 tokens, 32 heads over 8, 391 against 363 us)
-extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8, false>(p); }
+extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_wide_d128)(AttnPagedParams p) { attn_paged_many<128, 8, 1, false>(p); }
 extern "C" __global__ void __launch_bounds__(512) GEMM_KERNEL(attn_paged_join_wide_d128)(AttnPagedParams p) { attn_paged_join<128, 256, false>(p); }
+extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_pair_d64)(AttnPagedParams p) { attn_paged_many<64, 4, 2, false>(p); }
+extern "C" __global__ void __launch_bounds__(512, 2) GEMM_KERNEL(attn_paged_pair_d128)(AttnPagedParams p) { attn_paged_many<128, 4, 2, false>(p); }

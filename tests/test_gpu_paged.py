@@ -922,3 +922,37 @@ def test_attention_paged_wide_groups_and_many_heads(gpu, stream, nh, nkvh):
 @pytest.mark.parametrize("nt,nh,nkh,dh", [(600, 6, 2, 128), (300, 2, 2, 64), (2100, 3, 1, 64)])
 def test_qk_norm_rope_in_place_with_several_tokens_per_workgroup(gpu, stream, nt, nh, nkh, dh):
     check_norm(gpu, stream, np.random.default_rng(49), nt, nh, nkh, dh, "f16", "f32", 10000.0, "in_place")
+
+
+# ---- tiles of 128 rows whose keys two groups of waves take in turn
+
+@pytest.mark.parametrize("mask", [1, 0])
+@pytest.mark.parametrize("lens", [[(1, 700), (3, 9), (0, 5)], [(300, 330)], [(17, 400), (1, 1500), (40, 40)], [(1100, 1100)], [(5, 2)] + [(1, 30)] * 66 + [(30, 600)],
+                                  [(20, 64), (20, 65), (20, 128), (20, 129), (33, 33), (20, 192)]],
+                         ids=["decode", "prompt", "mixed", "long", "many", "edges"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_in_two_groups(gpu, stream, monkeypatch, lens, mask, dh):
+    test_attention_paged_every_size_of_tile(gpu, stream, monkeypatch, "3", lens, mask, dh)
+
+
+@pytest.mark.parametrize("form", ["token_major", "head_gap", "fused_qkv", "o_over_q", "strided_batch", "unlike_caches", "descending"])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_views_in_two_groups(gpu, stream, monkeypatch, form, dh):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", "3")
+    test_attention_paged_views(gpu, stream, form, (4, 2, dh, 16, [(50, 290), (1, 40), (3, 3), (20, 1500)]))
+
+
+@pytest.mark.parametrize("slots", ["1", "3", "40"])
+def test_attention_paged_key_ranges_in_two_groups(gpu, stream, monkeypatch, slots):
+    test_attention_paged_few_and_many_key_ranges(gpu, stream, monkeypatch, "3", slots)
+
+
+@pytest.mark.parametrize("kind,value", [("f16", np.nan), ("bf16", np.inf)])
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_paged_what_is_masked_does_not_matter_in_two_groups(gpu, stream, monkeypatch, kind, value, dh):
+    test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, "3", kind, value, dh)
+
+
+def test_attention_paged_hard_batches_in_two_groups(gpu, stream, monkeypatch):
+    test_attention_paged_hard_batches_on_large_tiles(gpu, stream, monkeypatch, "3")
+    test_attention_paged_many_sequences_on_every_tile(gpu, stream, monkeypatch, 600, "3")
