@@ -517,8 +517,8 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
  * (the same view), otherwise the address ranges of o and of q or the caches must not overlap (ArgsNotSupport).
  * What a row does not see does not touch it, infinite and NaN keys and values included.  Sums and softmax statistics are
  * f32; the result is rounded once, and in f16 and bf16 so are the probabilities of sequences with more than 16 rows
- * (new tokens times query heads per kv head).  Fast for f16 and bf16 with dh a multiple of 8 up to 256 and
- * rows that start on 16 bytes; other calls are right, but not fast. */
+ * (new tokens times query heads per kv head).  Fast for f16 and bf16 with dh a multiple of 8 and f32
+ * with dh a multiple of 4, up to 256, and rows that start on 16 bytes; other calls are right, but not fast. */
 typedef struct ophip_attention_paged_args {
     ophip_tensor_layout q_layout;
     const void *q_base;

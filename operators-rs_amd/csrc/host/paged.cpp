@@ -127,6 +127,7 @@ PagedBatch batch_params(const BatchMeta &m, size_t nt, const ophip_tensor_layout
 // ============================================================== attention_paged ===
 
 struct ophip_attention_paged : OpBase {
+    hipFunction_t f32[3];        // [dh up to 64, 128, 256]: tiles of 64 rows
     hipFunction_t any[3][4][2];  // [type][dh up to 64, 128, 256, 512][4 / 16 waves]
     // [f16 / bf16][tiles of 16 / 128 / 256 / 128 rows for two groups][dh 64, 128, below 64, below 128, up to 256]; 256 rows for dh 128
     // only, two groups for 64 and 128
@@ -135,6 +136,7 @@ struct ophip_attention_paged : OpBase {
     // one kind of tile (1 where there is no other for the head dimension)
     int slots = 0, tile = -1;
     explicit ophip_attention_paged(ophip_device *d) : OpBase(d) {
+        for (int n = 0; n < 3; ++n) f32[n] = d->kernel("attention_paged_f32", ("attn_paged_f32_d" + std::to_string(64 << n)).c_str());
         static const char *const tag[3] = {"f16", "bf16", "f32"};
         for (int t = 0; t < 3; ++t)
             for (int n = 0; n < 4; ++n)
@@ -272,10 +274,11 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     p.group = make_fastdiv((uint32_t)(nh / nkvh));
     p.nkvh = (uint32_t)nkvh, p.dh = (uint32_t)dh, p.causal = a.mask == OPHIP_MASK_CAUSAL;
     p.scale = scale;
+    const bool vec = vector_rows(a.q_layout, a.q_base) && vector_rows(a.o_layout, a.o_base) && vector_rows(a.k_cache_layout, a.k_cache_base) &&
+                     vector_rows(a.v_cache_layout, a.v_cache_base);
     const AttnPagedPlan plan = attention_paged_plan(op, m);
     // (a scale that is not positive: the matrix kernels take the maximum before they scale)
-    if (plan.matrix && p.b.cols && scale > 0.f && plan.grid <= 0xffffffffu / 512 && vector_rows(a.q_layout, a.q_base) && vector_rows(a.o_layout, a.o_base) &&
-        vector_rows(a.k_cache_layout, a.k_cache_base) && vector_rows(a.v_cache_layout, a.v_cache_base)) {
+    if (plan.matrix && p.b.cols && scale > 0.f && plan.grid <= 0xffffffffu / 512 && vec) {
         Workspace ws(qa, workspace, workspace_len, plan.workspace);
         p.work = ws.ptr();
         p.slots = (uint32_t)plan.slots;
@@ -290,6 +293,16 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         return;
     }
     op->dev->make_current();
+    // f32: tiles of 64 rows on the matrix cores from 16 rows per sequence on, which are a wave's, or from four where there are two
+    // tiles for each CU (heads of 128, 32 over 8, over 2000 to 4000 keys: 16 sequences of 16 rows 294 us against 516 a row at
+    // a time, 64 of four 463 against 636; 32 of four 455 against 420).
+    const size_t rows = nt * (nh / nkvh), units = nkvh * ((rows + std::min(nseq, nt) * 63) / 64);
+    const bool tiles = op->tile >= 0 ? op->tile > 0
+                                     : rows >= 16 * nseq || (rows >= 4 * nseq && dh <= 128 && nkvh * nseq >= 2 * (size_t)op->dev->props.multiProcessorCount);
+    if (m.dt == OPHIP_DT_F32 && dh % 4 == 0 && dh <= 256 && p.b.cols && vec && units <= 0xffffffffu / 256 && tiles) {
+        launch(op->f32[dh <= 64 ? 0 : dh <= 128 ? 1 : 2], Dim3{(unsigned)units}, Dim3{256}, 0, stream_of(qa), p);
+        return;
+    }
     // sixteen waves to a row where there are no more than two rows to a CU
     const int n = dh <= 64 ? 0 : dh <= 128 ? 1 : dh <= 256 ? 2 : 3, w = nt * nh <= 2 * (size_t)op->dev->props.multiProcessorCount;
     launch(op->any[type_index(m.dt)][n][w], Dim3{(unsigned)nt, (unsigned)nh}, Dim3{w ? 1024u : 256u}, 0, stream_of(qa), p);

@@ -265,6 +265,18 @@ inline cpusim_f32x4 cpusim_mfma_16x16x32(int line, V a, V b, cpusim_f32x4 c) {
 }
 #define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, x, y, z) cpusim_mfma_16x16x32<cpusim_f16x8>(__LINE__, a, b, c)
 #define __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, x, y, z) cpusim_mfma_16x16x32<cpusim_bf16x8>(__LINE__, a, b, c)
+// v_mfma_f32_16x16x4_f32: D[16 x 16] = A[16 x 4] . B[4 x 16] + C.  Lane l holds A[l % 16][l / 16], B[l / 16][l % 16] and D as above.
+inline cpusim_f32x4 cpusim_mfma_16x16x4(int line, float a, float b, cpusim_f32x4 c) {
+    const cpusim::WaveView w = cpusim::wave_exchange((uint32_t)line, &a, 4, &b, 4);
+    const uint32_t lane = cpusim::lane_id(), j = lane % 16, i0 = 4 * (lane / 16);
+    for (int q = 0; q < 4; ++q) {
+        float acc = c[q];
+        for (uint32_t g = 0; g < 4; ++g) acc += *reinterpret_cast<const float *>(w.a[g * 16 + i0 + q]) * *reinterpret_cast<const float *>(w.b[g * 16 + j]);
+        c[q] = acc;
+    }
+    return c;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, x, y, z) cpusim_mfma_16x16x4(__LINE__, a, b, c)
 // v_mfma_f32_32x32x16_{f16,bf16}: D[32 x 32] = A[32 x 16] . B[16 x 32] + C.  Lane l holds A[l % 32][8 (l / 32) ..+8],
 // B[8 (l / 32) ..+8][l % 32] and D[8 (r / 4) + 4 (l / 32) + r % 4][l % 32], r = 0 .. 15.
 template <class V>

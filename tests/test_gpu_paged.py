@@ -956,3 +956,51 @@ def test_attention_paged_what_is_masked_does_not_matter_in_two_groups(gpu, strea
 def test_attention_paged_hard_batches_in_two_groups(gpu, stream, monkeypatch):
     test_attention_paged_hard_batches_on_large_tiles(gpu, stream, monkeypatch, "3")
     test_attention_paged_many_sequences_on_every_tile(gpu, stream, monkeypatch, 600, "3")
+
+
+# ---- f32 on the matrix cores
+
+@pytest.mark.parametrize("mask", [1, 0])
+@pytest.mark.parametrize("lens", [[(1, 700), (3, 9), (0, 5)], [(300, 330)], [(17, 400), (1, 1500), (40, 40)], [(5, 2)] + [(1, 30)] * 66 + [(30, 600)],
+                                  [(20, 32), (20, 33), (16, 64), (15, 65), (33, 33), (1, 0), (8, 96)]],
+                         ids=["decode", "prompt", "mixed", "many", "edges"])
+@pytest.mark.parametrize("dh", [4, 36, 64, 100, 128, 200, 256])
+def test_attention_paged_f32_on_the_matrix_cores(gpu, stream, monkeypatch, lens, mask, dh):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", "1")
+    b = Batch(gpu, np.random.default_rng(50), "f32", 4, 2, dh, 24, lens, pad=1, head_gap=4)
+    want, tol = b.expected(mask)
+    check(attend(gpu, stream, b, mask), want, tol)
+
+
+@pytest.mark.parametrize("tile", ["0", "1"])
+@pytest.mark.parametrize("dh", [64, 100, 256])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_attention_paged_f32_what_is_masked_does_not_matter(gpu, stream, monkeypatch, tile, dh, value):
+    test_attention_paged_what_is_masked_does_not_matter(gpu, stream, monkeypatch, tile, "f32", value, dh)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
+@pytest.mark.parametrize("form", ["apart", "o_over_q", "tokens_first"])
+def test_attention_paged_f32_scales_and_views(gpu, stream, monkeypatch, scale, form):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", "1")
+    b = Batch(gpu, np.random.default_rng(51), "f32", 6, 2, 96, 16, [(40, 90), (9, 9), (1, 300)], pad=2, token_major=form == "tokens_first")
+    want, tol = b.expected(1, scale)
+    if form != "o_over_q":
+        return check(attend(gpu, stream, b, 1, scale=scale), want, tol)
+    q = b.q.view(b.q.host.transpose(1, 0, 2))
+    want[b.start[-1]:] = decode(b.q.host, "f32")[b.start[-1]:]
+    run(gpu, stream, ophip.AttentionPagedArgs(*q, *b.cache_args(), *q, *b.batch_args(), 1, scale))
+    check(decode(b.q.back(stream), "f32"), want, tol)
+
+
+def test_attention_paged_f32_hard_batches(gpu, stream, monkeypatch):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", "1")
+    b = Batch(gpu, np.random.default_rng(52), "f32", 4, 1, 128, 16, [(40, 60), (1, 300)])
+    b.q = Buffer(gpu, b.q.host * np.float32(20), "f32")
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
+    b = Batch(gpu, np.random.default_rng(53), "f32", 4, 2, 64, 16, [(40, 60), (1, 300), (20, 20)], junk=0.0)
+    for start, length in (([0, 1, 2, 0xFFFFFFFF], [50, 0xFFFFFFFF, 9]), ([5, 3, 1, 0], [50, 300, 9]), ([0, 0xFFFFFFF0, 0, 0xFFFFFFFF], [1, 1, 1])):
+        b.table = Buffer(gpu, np.full_like(b.table.host, 0x7FFFFFF0))
+        b.q_start, b.kv_len = Buffer(gpu, np.array(start, np.uint32)), Buffer(gpu, np.array(length, np.uint32))
+        attend(gpu, stream, b, 1)
