@@ -108,12 +108,14 @@ __device__ __forceinline__ void attn_paged_any(const AttnPagedParams &p) {
     __syncthreads();
     float top = s_m[0];
     for (int w = 1; w < WAVES; ++w) top = fmaxf(top, s_m[w]);
+    // (a wave without keys has a maximum of -inf, zeros beside it and no weight; one whose scores are all NaN has NaN beside it, which stays)
+    const float ref = top == -INFINITY ? 0.f : top;
     float total = 0.f;
-    for (int w = 0; w < WAVES; ++w) total += s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - top) * s_l[w];
+    for (int w = 0; w < WAVES; ++w) total += expf(s_m[w] - ref) * s_l[w];
     char *orow = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)token * p.o_st;
     for (uint32_t e = threadIdx.x; e < p.dh; e += WAVES * WAVE) {
         float x = 0.f;
-        for (int w = 0; w < WAVES; ++w) x += s_m[w] == -INFINITY ? 0.f : expf(s_m[w] - top) * s_o[w][e];
+        for (int w = 0; w < WAVES; ++w) x += expf(s_m[w] - ref) * s_o[w][e];
         // a row that keeps no key is zero
         *reinterpret_cast<T *>(orow + (int64_t)e * p.o_sd) = (T)(keep ? x / total : 0.f);
     }

@@ -1004,3 +1004,32 @@ def test_attention_paged_f32_hard_batches(gpu, stream, monkeypatch):
         b.table = Buffer(gpu, np.full_like(b.table.host, 0x7FFFFFF0))
         b.q_start, b.kv_len = Buffer(gpu, np.array(start, np.uint32)), Buffer(gpu, np.array(length, np.uint32))
         attend(gpu, stream, b, 1)
+
+
+# ---- values that are not finite where a row sees them
+
+def with_values(gpu, b, values):
+    """The batch with single elements of its caches replaced: (0: k, 1: v; sequence, key, head, column or slice, value)."""
+    for which, s, key, head, col, value in values:
+        b.cache_views[which][b.table.host[s, key // b.page], head, key % b.page, col] = encode(np.array([value]), b.kind)[0]
+    b.cache = [Buffer(gpu, c.host, b.kind) for c in b.cache]
+    b.cache_views = [c.host for c in b.cache]
+    return b
+
+
+EVERY_KERNEL = [("f16", 64, "0"), ("f16", 64, "1"), ("bf16", 64, "3"), ("bf16", 128, "0"), ("f16", 128, "1"), ("bf16", 128, "2"), ("f16", 128, "3"), ("f16", 96, "0"),
+                ("bf16", 200, "1"), ("bf16", 36, "0"), ("f16", 500, "0"), ("f32", 64, "0"), ("f32", 128, "0"), ("f32", 100, "1"), ("f32", 256, "1")]
+
+
+@pytest.mark.parametrize("kind,dh,tile", EVERY_KERNEL)
+@pytest.mark.parametrize("heads", [2, 40])
+def test_attention_paged_a_key_that_is_nan_is_not_dropped(gpu, stream, monkeypatch, kind, dh, tile, heads):
+    """NaN in the newest key, which one wave may hold alone, or in the first: every row that sees it is NaN."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(60), kind, heads, 1, dh, 16, [(1, 9), (1, 17), (1, 65), (1, 129), (1, 1), (2, 33), (1, 40), (20, 81)])
+    with_values(gpu, b, [(0, s, l - 1, 0, 0, np.nan) for s, (_, l) in enumerate(b.lens) if s != 6] + [(0, 6, 0, 0, 0, np.nan)])
+    for mask in (1, 0):
+        gpu.upload(b.o.mem, b.o.host)
+        want, tol = b.expected(mask)
+        assert np.isnan(want).any(-1).sum() >= 8 * heads
+        check(attend(gpu, stream, b, mask), want, tol, "mask %d" % mask)
