@@ -513,7 +513,8 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
 
 /* attention of the new tokens over the cache: o = softmax(scale * q . k^T) . v, q and o [nh, nt, dh], nh a multiple of
  * nkvh (query head h reads kv head h / (nh / nkvh)).  With OPHIP_MASK_CAUSAL new token i of n sees the keys up to its
- * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero.  q is left alone; o may be q itself
+ * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero; one that sees keys, all of them with a score of
+ * -inf, is NaN, as 0 / 0 is.  q is left alone; o may be q itself
  * (the same view), otherwise the address ranges of o and of q or the caches must not overlap (ArgsNotSupport).
  * What a row does not see does not touch it, infinite and NaN keys and values included.  Sums and softmax statistics are
  * f32; the result is rounded once, and in f16 and bf16 so are the probabilities of sequences with more than 16 rows

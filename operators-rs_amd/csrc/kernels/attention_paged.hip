@@ -90,7 +90,7 @@ __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const Pa
             if (lane == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + r) * 2) = f32x2{m, l};
         } else {
             elem *dst = reinterpret_cast<elem *>(reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st) + c0;
-            const float inv = l == 0.f ? 0.f : 1.0f / l;
+            const float inv = keep ? 1.0f / l : 0.f;  // (no key: zeros; no score above -inf: 0 / 0, as the definition has it)
 #pragma unroll
             for (int i = 0; i < W; ++i) dst[i] = f2e(o[i] * inv);
         }
@@ -303,7 +303,7 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
         if (column == 0) *reinterpret_cast<f32x2 *>(paged_stats(p) + ((size_t)it.slot * ROWS + j) * 2) = f32x2{top, total};
         return;
     }
-    const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
+    const float inv = keep ? 1.0f / total : 0.f;  // (no key: zeros; no score above -inf: 0 / 0)
     union {
         elem e[CW];
         uint32_t u[CW / 2];
@@ -599,7 +599,7 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
         return;
     }
     // two quads of a query are adjacent in lanes l and l + 32: one of each pair goes over, so that a lane stores 16 bytes
-    const float inv = total == 0.f ? 0.f : 1.0f / total;  // (nothing kept: zeros)
+    const float inv = lim ? 1.0f / total : 0.f;  // (no key: zeros; no score above -inf: 0 / 0)
     char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 16 * h;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -664,8 +664,8 @@ __device__ __forceinline__ void attn_paged_join(const AttnPagedParams &p) {
             }
             top = now;
         }
-        const float inv = total == 0.f ? 0.f : 1.0f / total;
         const uint32_t row = d.row0 + r, token = fastdiv(row, p.group), head = d.kvh * p.group.d + (row - token * p.group.d);
+        const float inv = token < d.blind ? 0.f : 1.0f / total;
         if (d.start >= p.b.nt || token >= p.b.nt - d.start) return;
         union {
             elem e[4];

@@ -194,7 +194,7 @@ __device__ __forceinline__ void attn_paged_f32(const AttnPagedParams &p) {
     l += __shfl_xor(l, 16, WAVE);
     l += __shfl_xor(l, 32, WAVE);
     if (wrow + j >= it.nrows) return;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;  // (nothing kept: zeros)
+    const float inv = lim ? 1.0f / l : 0.f;  // (no key: zeros; no score above -inf: 0 / 0)
     char *dst = reinterpret_cast<char *>(p.o) + (int64_t)head * p.o_sh + (int64_t)(it.s.start + token) * p.o_st + 64 * g;
 #pragma unroll
     for (int d = 0; d < DB; d += 4)

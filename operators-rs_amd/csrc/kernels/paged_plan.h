@@ -7,7 +7,7 @@
 // ---- the workspace: a count, a descriptor per slot (32 bytes), then per slot ROWS pairs (maximum, sum), then per slot
 // ROWS rows of DH floats
 struct PagedDesc {
-    uint32_t piece, pieces, kvh, row0, nrows, start, _pad[2];
+    uint32_t piece, pieces, kvh, row0, nrows, start, blind, _pad;  // blind: the sequence's first tokens, that see no key
 };
 __device__ __forceinline__ PagedDesc *paged_desc(const AttnPagedParams &p) { return reinterpret_cast<PagedDesc *>(reinterpret_cast<char *>(p.work) + 64); }
 __device__ __forceinline__ float *paged_stats(const AttnPagedParams &p) { return reinterpret_cast<float *>(reinterpret_cast<char *>(p.work) + 64 + 32 * (size_t)p.slots); }
@@ -155,7 +155,10 @@ __device__ __forceinline__ bool paged_item(const AttnPagedParams &p, PagedItem &
     it.piece = rest - back * it.pieces;
     it.row0 = (tiles - 1 - back) * ROWS;
     it.nrows = min((uint32_t)ROWS, rows - it.row0);
-    if (it.pieces > 1 && tid == 0) paged_desc(p)[it.slot] = PagedDesc{it.piece, it.pieces, it.kvh, it.row0, it.nrows, it.s.start, {0, 0}};
+    if (it.pieces > 1 && tid == 0) {
+        const uint32_t blind = p.causal && it.s.n > it.s.len ? it.s.n - it.s.len : 0;
+        paged_desc(p)[it.slot] = PagedDesc{it.piece, it.pieces, it.kvh, it.row0, it.nrows, it.s.start, blind, 0};
+    }
     return true;
 }
 

@@ -1033,3 +1033,24 @@ def test_attention_paged_a_key_that_is_nan_is_not_dropped(gpu, stream, monkeypat
         want, tol = b.expected(mask)
         assert np.isnan(want).any(-1).sum() >= 8 * heads
         check(attend(gpu, stream, b, mask), want, tol, "mask %d" % mask)
+
+
+@pytest.mark.parametrize("kind,dh,tile", EVERY_KERNEL)
+@pytest.mark.parametrize("heads", [2, 18])
+def test_attention_paged_rows_whose_scores_are_all_minus_infinity(gpu, stream, monkeypatch, kind, dh, tile, heads):
+    """A softmax over scores of -inf alone is NaN; zeros are for rows that see no key.  One such key, several, all of a long
+    sequence whose keys are cut into ranges, and one that is all but the last; beside them rows that see nothing."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    lens = [(1, 1), (1, 40), (3, 70), (1, 1500), (9, 1100), (5, 3), (30, 20), (1, 90), (1, 0), (9, 1090)]
+    b = Batch(gpu, np.random.default_rng(61), kind, heads, 1, dh, 16, lens)
+    q = np.abs(decode(b.q.host, kind)) + 0.25
+    b.q = Buffer(gpu, encode(q, kind), kind)
+    low = [(0, s, j, 0, 0, -np.inf) for s, (_, l) in enumerate(lens) for j in range(l) if s != 9 and not (s == 7 and j == 89)]
+    with_values(gpu, b, low)
+    for mask in (1, 0):
+        gpu.upload(b.o.mem, b.o.host)
+        with np.errstate(invalid="ignore"):
+            want, tol = b.expected(mask)
+        assert np.isnan(want).any() and np.isfinite(want[b.start[9]:]).all()
+        assert not mask or (want[b.start[5]:b.start[5] + 2] == 0).all() and np.isnan(want[b.start[5] + 2]).all()
+        check(attend(gpu, stream, b, mask), want, tol, "mask %d" % mask)
