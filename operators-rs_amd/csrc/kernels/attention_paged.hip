@@ -52,9 +52,12 @@ __device__ __forceinline__ bool not_finite(uint32_t most) {
 }
 
 // The matrix kernels multiply the values of a tile's keys with a probability of zero where a row does not keep them, and
-// zero times infinity or NaN is NaN.  Where they have met values that are not finite in a tile that some row keeps in part
-// (the last ones under a causal mask), they come here for the whole range instead of handing out their result: a
-// wave to a row, key by key, as in attention_paged_any.hip.  What a row does not keep then does not touch it, whatever it is.
+// zero times infinity or NaN is NaN.  Where paged_many has met values that are not finite in a tile that some row keeps in part
+// (the last ones under a causal mask), and where paged_few's sums are not finite, they come here for the whole range instead
+// of handing out their result: a wave to a row, key by key, as in attention_paged_any.hip.  What a row does not keep then
+// does not touch it, whatever it is.  Right, but slow, a row and key at a time: an infinite value at the end of one of 47 decode
+// steps 530 us against 122 for all of them, of a prompt of 546 tokens among seven 0.9 ms against 29 us, of 511 tokens over 32511
+// keys 121 ms against 0.34.
 template <int DH, int ROWS, bool PAD>
 __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const PagedItem &it, uint32_t key0, uint32_t key1, uint32_t waves) {
     constexpr int W = DH / WAVE;  // columns per lane
@@ -120,7 +123,7 @@ struct FewTile {  // 32 keys
 template <int DH>
 struct FewLds {
     float m[4][16], l[4][16], o[4][DH / 4][WAVE];
-    uint32_t bad[4];  // by wave: values that are not finite, in a step that some row keeps in part
+    uint32_t bad[4];  // by wave: sums of values that are not finite, of a row whose probabilities are
 };
 
 // ROWS: of the tiles whose partial results the workspace holds
@@ -181,19 +184,13 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     f32x4 o[CW];
 #pragma unroll
     for (int t = 0; t < CW; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const uint32_t keep_first = paged_keep(p, it, fastdiv(it.row0, p.group));  // the tile's first row keeps the fewest
-    bool spoiled = false;
     auto multiply = [&](FewTile<CW> &t, uint32_t step) {
-        if (step * 32 + 32 > keep_first) {  // some rows do not keep some keys
-            uint32_t most = 0;
+        if (step * 32 + 32 > it.s.len) {  // (behind the last key: that key again)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int d = 0; d < CW / 2; ++d) {
-                    if (step * 32 + 16 * (i / 4) + 4 * g + i % 4 >= it.s.len) t.v[i][d] = 0;  // (the last key again)
-                    most = exponents(most, t.v[i][d]);
-                }
-            spoiled |= __builtin_amdgcn_ballot_w64(not_finite(most)) != 0;
+                for (int d = 0; d < CW / 2; ++d)
+                    if (step * 32 + 16 * (i / 4) + 4 * g + i % 4 >= it.s.len) t.v[i][d] = 0;
         }
         float x[8], mx = -INFINITY;
 #pragma unroll
@@ -268,6 +265,14 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
     }
     l += __shfl_xor(l, 16, WAVE);
     l += __shfl_xor(l, 32, WAVE);
+    // A value that is not finite has made NaN of its column here even in rows that do not keep it (zero times infinity), and in those that do,
+    // where a probability's rest is zero or negative.  (A sum that is NaN makes the whole row NaN: nothing to mend.)
+    bool bad = false;
+#pragma unroll
+    for (int c = 0; c < CW; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bad = bad || !(fabsf(o[c][i]) < INFINITY);
+    const bool spoiled = __builtin_amdgcn_ballot_w64(bad && l < INFINITY) != 0;
 
     // the four waves' results, on one maximum
     if (g == 0) lds.m[wave][j] = m, lds.l[wave][j] = l;

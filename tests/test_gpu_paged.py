@@ -1054,3 +1054,22 @@ def test_attention_paged_rows_whose_scores_are_all_minus_infinity(gpu, stream, m
         assert np.isnan(want).any() and np.isfinite(want[b.start[9]:]).all()
         assert not mask or (want[b.start[5]:b.start[5] + 2] == 0).all() and np.isnan(want[b.start[5] + 2]).all()
         check(attend(gpu, stream, b, mask), want, tol, "mask %d" % mask)
+
+
+@pytest.mark.parametrize("kind,dh,tile", EVERY_KERNEL)
+@pytest.mark.parametrize("heads", [2, 18])
+def test_attention_paged_infinite_values_that_a_row_sees(gpu, stream, monkeypatch, kind, dh, tile, heads):
+    """An infinite value makes its column infinite, of its sign, and two of unlike signs NaN; the other columns are as ever."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(62), kind, heads, 1, dh, 16, [(1, 90), (1, 1), (3, 200), (1, 1500), (9, 150), (1, 300), (30, 140)])
+    with_values(gpu, b, [(1, 0, 20, 0, 3, np.inf), (1, 0, 5, 0, 7, -np.inf), (1, 1, 0, 0, 1, np.inf), (1, 2, 40, 0, 0, -np.inf), (1, 2, 100, 0, 0, -np.inf),
+                         (1, 3, 700, 0, dh - 1, np.inf), (1, 4, 64, 0, 9, np.inf), (1, 5, 3, 0, 2, np.inf), (1, 5, 130, 0, 2, -np.inf), (1, 6, 10, 0, 12, np.inf)])
+    for mask in (1, 0):
+        gpu.upload(b.o.mem, b.o.host)
+        with np.errstate(invalid="ignore"):
+            want, tol = b.expected(mask)
+        got = attend(gpu, stream, b, mask)
+        off = ~np.isfinite(want)
+        assert off.sum() == heads * (2 + 1 + 3 + 1 + 9 + 1 + 30)
+        assert np.array_equal(got[off], want[off], equal_nan=True), "mask %d" % mask
+        check(got, want, tol, "mask %d" % mask)
