@@ -507,7 +507,7 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
  *                    kv_len[s] - n + i.  Tokens in front of the first and behind the last sequence belong to none: their
  *                    rows are neither read nor written.
  * Table, starts and lengths are device data that may change between replays of a recorded launch.  The kernels bound
- * what they take from them: token numbers by nt, lengths by cols * page; a page number that is none of the cache's
+ * what they take from them: token numbers by nt, lengths by cols * page (attention) or keys (append); a page number that is none of the cache's
  * gets nothing written to, and reads as some page of the cache.  Wrong data gives wrong rows, not stray accesses.
  * Types: f16, bf16, f32, one for all tensors of a call.  dh up to 512. */
 
@@ -550,8 +550,8 @@ OPHIP_API void ophip_attention_paged_destroy(ophip_attention_paged *op);
 /* The new tokens' k and v [nkvh, nt, dh] into the cache, k rotated by rope (adjacent pairs, angle
  * p * theta^(-2 i / dh)) on the way; theta = 0: as they are, and p is not read.  p [nt] u32, u64, i32 or i64 holds the
  * tokens' positions, none negative.  A token whose key number is negative (kv_len less than the number of new tokens)
- * is not written.  k and v must not overlap the caches (ArgsNotSupport); two tokens with the same place in the cache
- * leave either one's row.  The angles are taken in f64: rope's, to f32 accuracy at any position. */
+ * or has no column of the table (kv_len beyond cols * page) is not written, and nothing else in its place.  k and v must not
+ * overlap the caches (ArgsNotSupport); two tokens with the same place in the cache leave parts of either one's row there.  The angles are taken in f64: rope's, to f32 accuracy at any position. */
 typedef struct ophip_kv_append_paged_args {
     ophip_tensor_layout k_layout;
     const void *k_base;

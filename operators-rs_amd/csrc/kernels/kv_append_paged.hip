@@ -10,13 +10,15 @@
 
 extern __shared__ float2 append_sc[];  // dh / 2 entries of (sin, cos)
 
-// Where the token's rows go: false when it belongs to no sequence, or its page is none of the cache's.
+// Where the token's rows go: false when it belongs to no sequence, or its key has no column of the table, or its page is none of the
+// cache's.  The key comes from the description as it stands: bounded by the table first, a length beyond it would move the
+// last tokens over keys that are there.
 __device__ __forceinline__ bool append_place(const KvAppendPagedParams &p, uint32_t token, uint32_t &page, uint32_t &row) {
     const uint32_t seq = paged_seq_of(p.b, token);
     if (seq >= p.b.nseq) return false;
-    const PagedSeq s = paged_seq(p.b, seq);
-    const int64_t key = (int64_t)s.len - s.n + (token - s.start);
-    if (token < s.start || token >= s.start + s.n || key < 0) return false;
+    const uint32_t start = paged_u32(p.b.q_start, (int64_t)seq * p.b.s_step), end = paged_u32(p.b.q_start, (int64_t)(seq + 1) * p.b.s_step);
+    const int64_t key = (int64_t)paged_u32(p.b.kv_len, (int64_t)seq * p.b.l_step) - end + token;  // len - (end - start) + (token - start)
+    if (token < start || token >= end || key < 0 || key >= (int64_t)(p.b.cols * p.b.page.d)) return false;
     const uint32_t col = fastdiv((uint32_t)key, p.b.page);
     page = paged_page(p.b, seq, col);
     row = (uint32_t)key - col * p.b.page.d;

@@ -1073,3 +1073,38 @@ def test_attention_paged_infinite_values_that_a_row_sees(gpu, stream, monkeypatc
         assert off.sum() == heads * (2 + 1 + 3 + 1 + 9 + 1 + 30)
         assert np.array_equal(got[off], want[off], equal_nan=True), "mask %d" % mask
         check(got, want, tol, "mask %d" % mask)
+
+
+# ---- appends to a cache that has no place for them
+
+@pytest.mark.parametrize("dh", [64, 6])
+@pytest.mark.parametrize("kv_type,over", [(np.uint32, [17, 40, 0xFFFFFFFF, 18]), (np.int32, [17, 33, -1, 16])])
+def test_kv_append_paged_beyond_the_table(gpu, stream, dh, kv_type, over):
+    """A sequence that has outgrown its row of the table: tokens whose key has no column are not written, those before them
+    are, and no row of the cache that was there changes."""
+    b = append_case(gpu, np.random.default_rng(63), "f16", 2, dh, 16, [(1, 16), (4, 16), (2, 16), (4, 16)], 1)
+    b.kv_len = Buffer(gpu, np.array(over, kv_type))
+    run(gpu, stream, append_args(b, 0.0), ophip.KvAppendPaged(gpu))
+    want = [c.host.copy() for c in b.cache]
+    for s, (n, _) in enumerate(b.lens):
+        for i in range(n):
+            key = int(over[s]) - n + i
+            if 0 <= key < 16:
+                assert s == 3
+                for w, x in zip(want, (b.k, b.v)):
+                    w[b.table.host[s, 0], :, key] = x.host[b.start[s] + i]
+    for c, w in zip(b.cache, want):
+        assert np.array_equal(c.back(stream).view(np.uint8), w.view(np.uint8))
+
+
+def test_kv_append_paged_a_sequence_that_ends_behind_the_batch(gpu, stream):
+    """q_start that names more tokens than there are: those that are there are the sequence's first, and get their keys."""
+    b = append_case(gpu, np.random.default_rng(64), "bf16", 2, 64, 16, [(3, 20), (2, 30)], 0)
+    b.q_start = Buffer(gpu, np.array([0, 3, 9], np.uint32))  # six tokens of the second sequence, two of them here: keys 24, 25
+    run(gpu, stream, append_args(b, 0.0), ophip.KvAppendPaged(gpu))
+    want = [c.host.copy() for c in b.cache]
+    for t, s, key in ((0, 0, 17), (1, 0, 18), (2, 0, 19), (3, 1, 24), (4, 1, 25)):
+        for w, x in zip(want, (b.k, b.v)):
+            w[b.table.host[s, key // 16], :, key % 16] = x.host[t]
+    for c, w in zip(b.cache, want):
+        assert np.array_equal(c.back(stream), w)
