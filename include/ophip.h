@@ -515,7 +515,7 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
  * nkvh (query head h reads kv head h / (nh / nkvh)).  With OPHIP_MASK_CAUSAL new token i of n sees the keys up to its
  * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero; one that sees keys, all of them with a score of
  * -inf, is NaN, as 0 / 0 is.  q is left alone; o may be q itself
- * (the same view), otherwise the address ranges of o and of q or the caches must not overlap (ArgsNotSupport).
+ * (the same view), otherwise the address ranges of o and of q, the caches, the table, the starts or the lengths must not overlap (ArgsNotSupport).
  * What a row does not see does not touch it, infinite and NaN keys and values included.  Sums and softmax statistics are
  * f32; the result is rounded once, and in f16 and bf16 so are the probabilities of sequences with more than 16 rows
  * (new tokens times query heads per kv head).  Fast for f16 and bf16 with dh a multiple of 8 and f32
@@ -550,8 +550,8 @@ OPHIP_API void ophip_attention_paged_destroy(ophip_attention_paged *op);
 /* The new tokens' k and v [nkvh, nt, dh] into the cache, k rotated by rope (adjacent pairs, angle
  * p * theta^(-2 i / dh)) on the way; theta = 0: as they are, and p is not read.  p [nt] u32, u64, i32 or i64 holds the
  * tokens' positions, none negative.  A token whose key number is negative (kv_len less than the number of new tokens)
- * or has no column of the table (kv_len beyond cols * page) is not written, and nothing else in its place.  k and v must not
- * overlap the caches (ArgsNotSupport); two tokens with the same place in the cache leave parts of either one's row there.  The angles are taken in f64: rope's, to f32 accuracy at any position. */
+ * or has no column of the table (kv_len beyond cols * page) is not written, and nothing else in its place.  k, v, p, the
+ * table, the starts and the lengths must not overlap the caches (ArgsNotSupport), and the caches must not share elements; two tokens with the same place in the cache leave parts of either one's row there.  The angles are taken in f64: rope's, to f32 accuracy at any position. */
 typedef struct ophip_kv_append_paged_args {
     ophip_tensor_layout k_layout;
     const void *k_base;
@@ -584,8 +584,8 @@ OPHIP_API void ophip_kv_append_paged_destroy(ophip_kv_append_paged *op);
  * y[t, h, :] = rope(x[t, h, :] / sqrt(mean(x[t, h, :]^2) + epsilon) * w, p[t]) with x = q, w = qw, y = qy and
  * x = k, w = kw, y = ky.  q, qy [nt, nh, dh], k, ky [nt, nkh, dh] (either may have no heads), dh even and contiguous;
  * qw, kw [dh] of the rows' type or f32; p and theta as in kv_append_paged (theta = 0: the norms alone).
- * qy may be q and ky may be k (the same view); otherwise a y that overlaps its x is ArgsNotSupport, and qy must not
- * share elements with k or ky. */
+ * qy may be q and ky may be k (the same view); otherwise a y that overlaps its x is ArgsNotSupport, and so is one that overlaps
+ * weights or positions; qy must not share elements with k or ky, nor ky with q. */
 typedef struct ophip_qk_norm_rope_args {
     ophip_tensor_layout qy_layout;
     void *qy_base;

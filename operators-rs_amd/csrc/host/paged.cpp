@@ -262,6 +262,9 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         throw args_not_support("o overlaps q");
     if (!apart(a.o_layout, a.o_base, a.k_cache_layout, a.k_cache_base) || !apart(a.o_layout, a.o_base, a.v_cache_layout, a.v_cache_base))
         throw args_not_support("o overlaps the cache");
+    if (!apart(a.o_layout, a.o_base, a.page_table_layout, a.page_table_base) || !apart(a.o_layout, a.o_base, a.q_start_layout, a.q_start_base) ||
+        !apart(a.o_layout, a.o_base, a.kv_len_layout, a.kv_len_base))
+        throw args_not_support("o overlaps the page table, q_start or kv_len");
     p.q = a.q_base, p.o = a.o_base, p.k = a.k_cache_base, p.v = a.v_cache_base;
     const ptrdiff_t *s = a.q_layout.strides;
     p.q_sh = s[0], p.q_st = s[1], p.q_sd = s[2];
@@ -390,14 +393,17 @@ void kv_append_paged_launch(const ophip_kv_append_paged *op, const ophip_kv_appe
     if (p.b.cols == 0) return;  // no place for any key
     if (nkvh > MAX_INDEX / MAX_HEAD) throw shape_not_support("too many heads");
     if (!a.k_base || !a.v_base || !a.k_cache_base || !a.v_cache_base || (p.rotate && !a.p_base)) throw args_not_support("null base address");
-    // a workgroup writes the cache while others still read k and v
+    // a workgroup writes the caches while others still read everything else
     const struct {
         const ophip_tensor_layout &l;
         const void *base;
-    } from[2] = {{a.k_layout, a.k_base}, {a.v_layout, a.v_base}};
-    for (const auto &f : from)
-        if (!apart(f.l, f.base, a.k_cache_layout, a.k_cache_base) || !apart(f.l, f.base, a.v_cache_layout, a.v_cache_base))
-            throw args_not_support("k or v overlaps the cache");
+    } from[6] = {{a.k_layout, a.k_base}, {a.v_layout, a.v_base}, {a.page_table_layout, a.page_table_base}, {a.q_start_layout, a.q_start_base},
+                 {a.kv_len_layout, a.kv_len_base}, {a.p_layout, a.p_base}};
+    for (int i = 0; i < (p.rotate ? 6 : 5); ++i)
+        if (!apart(from[i].l, from[i].base, a.k_cache_layout, a.k_cache_base) || !apart(from[i].l, from[i].base, a.v_cache_layout, a.v_cache_base))
+            throw args_not_support(i < 2 ? "k or v overlaps the cache" : "the page table, q_start, kv_len or p overlaps the cache");
+    // (the caches' address ranges may meet, as those of two halves of one buffer do, their elements not)
+    if (a.k_cache_base == a.v_cache_base) throw args_not_support("k_cache and v_cache are one");
     p.k = a.k_base, p.v = a.v_base, p.pos = a.p_base, p.k_cache = a.k_cache_base, p.v_cache = a.v_cache_base;
     const ptrdiff_t *s = a.k_layout.strides;
     p.k_sh = s[0], p.k_st = s[1], p.k_sd = s[2];
@@ -526,6 +532,15 @@ void qk_norm_rope_launch(const ophip_qk_norm_rope *op, const ophip_qk_norm_rope_
         vec = vec && vector_rows(h.y, h.y_base) && vector_rows(h.x, h.x_base);
     }
     if (p.rotate && !a.p_base) throw args_not_support("null base address");
+    // a workgroup writes its rows while others still read weights, positions and the other rows
+    for (int i = 0; i < 2; ++i) {
+        const auto &h = half[i], &other = half[1 - i];
+        if (h.nh == 0) continue;
+        if (!apart(h.y, h.y_base, h.w, h.w_base) || (other.nh && !apart(h.y, h.y_base, other.w, other.w_base)) || (p.rotate && !apart(h.y, h.y_base, a.p_layout, a.p_base)))
+            throw args_not_support("y overlaps weights or positions");
+        // (the ranges of q's and k's rows may meet, as those of one projection's parts do, their elements not)
+        if (other.nh && (h.y_base == other.y_base || h.y_base == other.x_base)) throw args_not_support("qy shares elements with k or ky, or ky with q");
+    }
     p.pos = a.p_base;
     p.p_step = a.p_layout.strides[0];
     p.pos_is_u64 = ophip_dtype_nbytes(a.p_layout.dt) == 8;

@@ -1108,3 +1108,79 @@ def test_kv_append_paged_a_sequence_that_ends_behind_the_batch(gpu, stream):
             w[b.table.host[s, key // 16], :, key % 16] = x.host[t]
     for c, w in zip(b.cache, want):
         assert np.array_equal(c.back(stream), w)
+
+
+# ---- results over what other workgroups still read
+
+def test_attention_paged_refuses_results_over_the_description(gpu, stream):
+    b = Batch(gpu, np.random.default_rng(65), "f16", 4, 2, 64, 16, [(1, 20), (2, 30)])
+    op = ophip.AttentionPaged(gpu)
+    for n in ("page_table_base", "q_start_base", "kv_len_base"):
+        a = b.args(1)
+        setattr(a, n, b.o.mem.ptr + 16)
+        with pytest.raises(ophip.LaunchError) as e:
+            op.launch(a, None, stream)
+        assert e.value.kind == "ArgsNotSupport", n
+    op.launch(b.args(1), None, stream)
+    stream.synchronize()
+
+
+def test_kv_append_paged_refuses_caches_over_what_it_reads(gpu, stream):
+    b = append_case(gpu, np.random.default_rng(66), "f16", 2, 64, 16, [(1, 20), (2, 30)], 0)
+    op = ophip.KvAppendPaged(gpu)
+    for which in (0, 1):
+        for n in ("page_table_base", "q_start_base", "kv_len_base", "p_base"):
+            a = append_args(b, 10000.0)
+            setattr(a, n, b.cache[which].mem.ptr + 16)
+            with pytest.raises(ophip.LaunchError) as e:
+                op.launch(a, None, stream)
+            assert e.value.kind == "ArgsNotSupport", n
+    a = append_args(b, 10000.0)
+    a.v_cache_base = a.k_cache_base  # one cache for both
+    with pytest.raises(ophip.LaunchError) as e:
+        op.launch(a, None, stream)
+    assert e.value.kind == "ArgsNotSupport"
+    a = append_args(b, 0.0)
+    a.p_base = b.cache[0].mem.ptr  # positions that are not read may lie anywhere
+    check_append(gpu, stream, b, 0.0, a)
+
+
+def test_kv_append_paged_caches_side_by_side_in_one_buffer(gpu, stream):
+    """Both caches in one buffer, k's and v's pages in turn: their address ranges meet, their elements do not."""
+    b = append_case(gpu, np.random.default_rng(67), "f16", 2, 64, 16, [(1, 20), (2, 30), (7, 7)], 0)
+    both = Buffer(gpu, np.stack([c.host for c in b.cache], 1), "f16")
+    a = append_args(b, 0.0)
+    (a.k_cache_layout, a.k_cache_base), (a.v_cache_layout, a.v_cache_base) = (both.view(both.host[:, i]) for i in (0, 1))
+    run(gpu, stream, a, ophip.KvAppendPaged(gpu))
+    got = both.back(stream)
+    check_append(gpu, stream, b, 0.0)
+    for i, c in enumerate(b.cache):
+        assert np.array_equal(got[:, i].view(np.uint8), c.back(stream).view(np.uint8))
+
+
+def test_qk_norm_rope_refuses_results_over_what_it_reads(gpu, stream):
+    op, mem = ophip.QkNormRope(gpu), gpu.malloc(1 << 16)
+    lay = lambda h: TensorLayout.new_contiguous(dt.F16, [2, h, 64])
+    w, p = TensorLayout.new_contiguous(dt.F16, [64]), TensorLayout.new_contiguous(dt.U32, [2])
+    base = lambda i: mem.ptr + 4096 * i
+
+    def make(theta=10000.0, **change):
+        a = ophip.QkNormRopeArgs(lay(4), base(0), lay(4), base(1), w, base(2), lay(2), base(3), lay(2), base(4), w, base(5), p, base(6), 1e-5, theta)
+        for k, v in change.items():
+            setattr(a, k, v)
+        return a
+
+    for y in (0, 3):
+        for n in ("qw_base", "kw_base", "p_base"):
+            with pytest.raises(ophip.LaunchError) as e:
+                op.launch(make(**{n: base(y) + 16}), None, stream)
+            assert e.value.kind == "ArgsNotSupport", n
+    for n in ("ky_base", "k_base"):  # the other rows' input or result: the same address
+        with pytest.raises(ophip.LaunchError) as e:
+            op.launch(make(**{n: base(0)}), None, stream)
+        assert e.value.kind == "ArgsNotSupport", n
+    with pytest.raises(ophip.LaunchError) as e:
+        op.launch(make(q_base=base(3)), None, stream)
+    assert e.value.kind == "ArgsNotSupport"
+    op.launch(make(theta=0.0, p_base=base(0)), None, stream)
+    stream.synchronize()
