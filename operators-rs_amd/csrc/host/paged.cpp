@@ -296,18 +296,21 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
         return;
     }
     op->dev->make_current();
-    // f32: tiles of 64 rows on the matrix cores from 16 rows per sequence on, which are a wave's, or from four where there are two
-    // tiles for each CU (heads of 128, 32 over 8, over 2000 to 4000 keys: 16 sequences of 16 rows 294 us against 516 a row at
-    // a time, 64 of four 463 against 636; 32 of four 455 against 420).
-    const size_t rows = nt * (nh / nkvh), units = nkvh * ((rows + std::min(nseq, nt) * 63) / 64);
-    const bool tiles = op->tile >= 0 ? op->tile > 0
-                                     : rows >= 16 * nseq || (rows >= 4 * nseq && dh <= 128 && nkvh * nseq >= 2 * (size_t)op->dev->props.multiProcessorCount);
+    // f32: tiles of 64 rows on the matrix cores where they are less work than a row at a time.  A tile's keys are never cut into
+    // ranges, so it takes a CU as long as `worth` rows, of which as many run at a time as there are CUs; fewer tiles than CUs
+    // take no less time for that.  1253 batches of 1 to 256 sequences and tokens, 512 to 32768 keys, heads 16 over 1 to 32 over 32:
+    // within 7 % of the faster one at dh 64, 13 % at 128, 27 % at 256.  Tiles against rows, dh 128: a step of 16 heads over 1 and
+    // 4096 keys 379 us, 109; 16 tokens, 32 heads over 8, 32768 keys 3.42 ms, 1.76; 64 tokens 3.45 ms, 5.88; 256 tokens, 4096 keys
+    // 0.41 ms, 2.59; 64 steps of 16 heads over 1, 32768 keys 3.71 ms, 3.64 (twice as many rows as CUs, three times would pay).
+    const size_t cus = (size_t)op->dev->props.multiProcessorCount, rows = nt * (nh / nkvh), units = nkvh * ((rows + std::min(nseq, nt) * 63) / 64);
+    const size_t worth = dh <= 64 ? 2 : dh <= 128 ? 3 : 5;
+    const bool tiles = op->tile >= 0 ? op->tile > 0 : nt * nh >= worth * std::max(units, cus);
     if (m.dt == OPHIP_DT_F32 && dh % 4 == 0 && dh <= 256 && p.b.cols && vec && units <= 0xffffffffu / 256 && tiles) {
         launch(op->f32[dh <= 64 ? 0 : dh <= 128 ? 1 : 2], Dim3{(unsigned)units}, Dim3{256}, 0, stream_of(qa), p);
         return;
     }
     // sixteen waves to a row where there are no more than two rows to a CU
-    const int n = dh <= 64 ? 0 : dh <= 128 ? 1 : dh <= 256 ? 2 : 3, w = nt * nh <= 2 * (size_t)op->dev->props.multiProcessorCount;
+    const int n = dh <= 64 ? 0 : dh <= 128 ? 1 : dh <= 256 ? 2 : 3, w = nt * nh <= 2 * cus;
     launch(op->any[type_index(m.dt)][n][w], Dim3{(unsigned)nt, (unsigned)nh}, Dim3{w ? 1024u : 256u}, 0, stream_of(qa), p);
 }
 

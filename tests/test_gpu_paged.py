@@ -1184,3 +1184,29 @@ def test_qk_norm_rope_refuses_results_over_what_it_reads(gpu, stream):
     assert e.value.kind == "ArgsNotSupport"
     op.launch(make(theta=0.0, p_base=base(0)), None, stream)
     stream.synchronize()
+
+
+# ---- which kernel f32 runs on
+
+@pytest.mark.parametrize("nh,nkvh,dh,lens,tiles", [
+    (16, 1, 128, [(1, 200)], False),            # one decode step whose 16 rows are a single tile
+    (32, 1, 64, [(1, 90), (1, 70)], False),
+    (8, 1, 256, [(9, 100)], False),
+    (4, 1, 64, [(16, 60)], False),              # 64 rows: one tile, or a workgroup for each
+    (12, 4, 64, [(50, 50)], True),              # 600 rows in 12 tiles
+    (16, 2, 128, [(49, 50)], True),             # 784 rows
+    (40, 1, 128, [(30, 40)], True),
+    (16, 2, 200, [(49, 50)], False),            # 784 rows: at this size a row at a time is still faster
+    (20, 1, 256, [(65, 65)], True),
+], ids=str)
+def test_attention_paged_f32_tiles_only_where_they_fill_the_machine(gpu, stream, monkeypatch, nh, nkvh, dh, lens, tiles):
+    """Tiles of 64 rows are never cut into ranges: few of them leave most CUs without work.  The chosen kernel shows in the
+    last bits: the two add in different orders."""
+    got = {}
+    b = Batch(gpu, np.random.default_rng(68), "f32", nh, nkvh, dh, 16, lens)
+    for tile in ("0", "1", None):
+        monkeypatch.delenv("OPHIP_ATTN_PAGED_TILE", raising=False) if tile is None else monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+        gpu.upload(b.o.mem, b.o.host)
+        got[tile] = attend(gpu, stream, b, 1)
+    assert not np.array_equal(got["0"], got["1"])
+    assert np.array_equal(got[None], got["1" if tiles else "0"])
