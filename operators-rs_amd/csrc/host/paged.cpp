@@ -298,7 +298,7 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     op->dev->make_current();
     // f32: tiles of 64 rows on the matrix cores where they are less work than a row at a time.  A tile's keys are never cut into
     // ranges, so it takes a CU as long as `worth` rows, of which as many run at a time as there are CUs; fewer tiles than CUs
-    // take no less time for that.  1253 batches of 1 to 256 sequences and tokens, 512 to 32768 keys, heads 16 over 1 to 32 over 32:
+    // take no less time for that.  1697 batches of 1 to 256 sequences and tokens, 64 to 32768 keys, heads 16 over 1 to 32 over 32:
     // within 7 % of the faster one at dh 64, 13 % at 128, 27 % at 256.  Tiles against rows, dh 128: a step of 16 heads over 1 and
     // 4096 keys 379 us, 109; 16 tokens, 32 heads over 8, 32768 keys 3.42 ms, 1.76; 64 tokens 3.45 ms, 5.88; 256 tokens, 4096 keys
     // 0.41 ms, 2.59; 64 steps of 16 heads over 1, 32768 keys 3.71 ms, 3.64 (twice as many rows as CUs, three times would pay).

@@ -1210,3 +1210,119 @@ def test_attention_paged_f32_tiles_only_where_they_fill_the_machine(gpu, stream,
         got[tile] = attend(gpu, stream, b, 1)
     assert not np.array_equal(got["0"], got["1"])
     assert np.array_equal(got[None], got["1" if tiles else "0"])
+
+
+# ---- what up to 16 rows promise: probabilities that are not rounded to the type
+
+@pytest.mark.parametrize("kind,dh,tile", [("f16", 64, "0"), ("bf16", 64, "1"), ("bf16", 128, "0"), ("f16", 128, "2"), ("bf16", 128, "3"), ("f16", 96, "0"), ("bf16", 256, "1"), ("f16", 8, "0")])
+@pytest.mark.parametrize("group", [4, 8])
+def test_attention_paged_decode_steps_do_not_round_probabilities(gpu, stream, monkeypatch, kind, dh, tile, group):
+    """Values of one sign over a few keys, so that roundings of probabilities do not cancel: within one rounding of the result.
+    A probability goes into the product as its rounding and the rounded rest, which leaves u^2 of it (in f16 no less than 2^-32
+    of the largest, 2^-27 for up to 32 keys), so the bound is u |o| + (u^2 + 2 (dh + 8) e S + 2^-20) A, with u, e, S and A as above.  Rounded
+    probabilities do not stay within it, which is computed here as well."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    rng = np.random.default_rng(70)
+    b = Batch(gpu, rng, kind, 2 * group, 2, dh, 16, [(1, int(l)) for l in rng.integers(2, 8, 40)] + [(16 // group, 20)])
+    b.cache = [b.cache[0], Buffer(gpu, encode(np.abs(decode(b.cache[1].host, kind)), kind), kind)]
+    b.cache_views = [c.host for c in b.cache]
+    b.q = Buffer(gpu, encode(decode(b.q.host, kind) * 0.25, kind), kind)  # small scores: what f32 leaves of them is little beside u
+    scale, u = float(np.float32(dh ** -0.5)), HALF[kind]
+    want, tol = np.zeros((b.nt, b.nh, dh)), np.zeros((b.nt, b.nh, dh))
+    q, rounded = decode(b.q.host, kind), np.zeros((b.nt, b.nh, dh))
+    for s, (n, l) in enumerate(b.lens):
+        k, v = b.keys(s, 0), b.keys(s, 1)
+        for i in range(n):
+            t, keep = b.start[s] + i, l - n + i + 1
+            for h in range(b.nh):
+                kk, vv = k[:keep, h // group], v[:keep, h // group]
+                x = kk @ q[t, h] * scale
+                p = np.exp(x - x.max())
+                big = (np.abs(kk) @ np.abs(q[t, h])).max() * scale
+                want[t, h] = p @ vv / p.sum()
+                tol[t, h] = u * np.abs(want[t, h]) + (u * u + 2 * (dh + 8) * E * big + 2.0 ** -20) * (p @ np.abs(vv) / p.sum()) + 2.0 ** -25
+                rounded[t, h] = decode(encode(decode(encode(p, kind), kind) @ vv / p.sum(), kind), kind)
+    assert (np.abs(rounded - want) > tol).sum() > 20
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+# ---- positions beyond 31 and 32 bits
+
+FAR = [(np.uint32, [0, 1, 0x7FFFFFFF, 0x80000000, 0xFFFFFFFF, 3000000019]), (np.int32, [0x7FFFFFFF, 2000000011]),
+       (np.uint64, [5, 1 << 32, (1 << 32) + 1, (1 << 33) + 12345, (1 << 40) - 1]), (np.int64, [7, (1 << 32) - 1, (1 << 35) + 977, 3 << 38])]
+
+
+def rotated_far(x, pos, theta):
+    """`rotated` with the angles in 80 bits, and what an angle computed in f64 may be off by: the exponent a of theta^(-k / half) = 2^-a
+    and its power are good to (a + 3) 2^-51 relative, rounding by rounding, and (a + 3) 2^-a <= 3: 3 pos 2^-51 radians."""
+    assert np.finfo(np.longdouble).nmant >= 63
+    half = x.shape[-1] // 2
+    freq = np.longdouble(np.float32(theta)) ** (-np.arange(half).astype(np.longdouble) / half)
+    ang = np.array([np.longdouble(int(p)) for p in pos])[:, None, None] * freq
+    c, s = np.cos(ang).astype(np.float64), np.sin(ang).astype(np.float64)
+    a, b = x[..., 0::2], x[..., 1::2]
+    out, size = np.empty_like(x), np.empty_like(x)
+    out[..., 0::2], out[..., 1::2] = a * c - b * s, a * s + b * c
+    size[..., 0::2] = size[..., 1::2] = np.abs(a) + np.abs(b)
+    return out, size * (2.0 ** -20 + 3 * 2.0 ** -51 * np.asarray(pos, np.float64)[:, None, None])
+
+
+@pytest.mark.parametrize("pos_type,far", FAR, ids=lambda x: np.dtype(x).name if isinstance(x, type) else "")
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dh", [64, 6])
+@pytest.mark.parametrize("theta", [10000.0, 500000.0])
+def test_kv_append_paged_angles_of_far_positions(gpu, stream, pos_type, far, kind, dh, theta):
+    n = len(far)
+    b = append_case(gpu, np.random.default_rng(71), kind, 2, dh, 16, [(n, n + 13)], 0)
+    b.pos = Buffer(gpu, np.array(far, pos_type))
+    run(gpu, stream, append_args(b, theta), ophip.KvAppendPaged(gpu))
+    want, tol = rotated_far(decode(b.k.host, kind), far, theta)
+    back = b.cache[0].back(stream)
+    got = np.array([decode(back[b.table.host[0, j // 16], :, j % 16], kind) for j in range(13, 13 + n)])
+    check(got, want, tol + HALF[kind] * np.abs(want) + 2.0 ** -25)
+
+
+@pytest.mark.parametrize("pos_type,far", FAR, ids=lambda x: np.dtype(x).name if isinstance(x, type) else "")
+@pytest.mark.parametrize("dh,many", [(64, 1), (6, 1), (128, 300)])
+def test_qk_norm_rope_angles_of_far_positions(gpu, stream, pos_type, far, dh, many):
+    """Rows of norm 1 before the rotation up to what the norm's own roundings leave; one token per workgroup and several."""
+    rng, theta = np.random.default_rng(72), 10000.0
+    far = (far * many)[:max(len(far), many)]
+    q, k = (Buffer(gpu, encode(rng.standard_normal((len(far), h, dh)), "f32"), "f32") for h in (3, 2))
+    qy, ky = (Buffer(gpu, np.zeros(x.host.shape, np.float32), "f32") for x in (q, k))
+    w, pos = Buffer(gpu, encode(1 + 0.2 * rng.standard_normal(dh), "f32"), "f32"), Buffer(gpu, np.array(far, pos_type))
+    run(gpu, stream, ophip.QkNormRopeArgs(*qy.view(), *q.view(), *w.view(), *ky.view(), *k.view(), *w.view(), *pos.view(), 1e-6, theta), ophip.QkNormRope(gpu))
+    for x, y in ((q, qy), (k, ky)):
+        x64 = x.host.astype(np.float64)
+        z = x64 / np.sqrt((x64 * x64).mean(-1, keepdims=True) + float(np.float32(1e-6))) * w.host.astype(np.float64)
+        want, tol = rotated_far(z, far, theta)
+        _, size = rotated(z, np.zeros(len(far)), theta)
+        check(y.back(stream).astype(np.float64), want, tol + size * (dh / 2 + 8) * E + HALF["f32"] * np.abs(want) + 2.0 ** -25)
+
+
+# ---- the plan of more sequences than a workgroup has threads, with key ranges
+
+@pytest.mark.parametrize("tile,dh", [("0", 64), ("1", 64), ("2", 128), ("3", 64)])
+@pytest.mark.parametrize("count", [65, 300, 1100])
+def test_attention_paged_key_ranges_among_many_sequences(gpu, stream, monkeypatch, count, tile, dh):
+    """Long sequences at the start, in the middle and at the end of many short ones: the sums that find a workgroup's place carry
+    over from round to round, tiles and ranges apart."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    rng = np.random.default_rng(73)
+    lens = [(int(n), int(l)) for n, l in zip(rng.integers(0, 3, count), rng.integers(0, 40, count))]
+    for s, n, l in ((0, 1, 1700), (1, 20, 1500), (count // 2, 1, 1600), (count // 2 + 1, 40, 1550), (count - 2, 9, 1580), (count - 1, 1, 1900)):
+        lens[s] = (n, l)
+    b = Batch(gpu, rng, "f16", 2, 1, dh, 32, lens, pad=2)
+    op = ophip.AttentionPaged(gpu)
+    assert op.scheme(b.args(1), 1 << 40) > 0
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1, op=op), want, tol)
+
+
+@pytest.mark.parametrize("slots", ["1", "3", "40"])
+def test_attention_paged_few_and_many_key_ranges_of_256_rows(gpu, stream, monkeypatch, slots):
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", "2")
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_SLOTS", slots)
+    b = Batch(gpu, np.random.default_rng(74), "bf16", 4, 2, 128, 16, [(20, 2000), (1, 3000), (150, 900)])
+    want, tol = b.expected(1)
+    check(attend(gpu, stream, b, 1), want, tol)
