@@ -297,14 +297,15 @@ void attention_paged_launch(const ophip_attention_paged *op, const ophip_attenti
     }
     op->dev->make_current();
     // f32: tiles of 64 rows on the matrix cores where they are less work than a row at a time.  A tile's keys are never cut into
-    // ranges, so it takes a CU as long as `worth` rows, of which as many run at a time as there are CUs; fewer tiles than CUs
-    // take no less time for that.  1697 batches of 1 to 256 sequences and tokens, 64 to 32768 keys, heads 16 over 1 to 32 over 32:
-    // within 7 % of the faster one at dh 64, 13 % at 128, 27 % at 256.  Tiles against rows, dh 128: a step of 16 heads over 1 and
-    // 4096 keys 379 us, 109; 16 tokens, 32 heads over 8, 32768 keys 3.42 ms, 1.76; 64 tokens 3.45 ms, 5.88; 256 tokens, 4096 keys
-    // 0.41 ms, 2.59; 64 steps of 16 heads over 1, 32768 keys 3.71 ms, 3.64 (twice as many rows as CUs, three times would pay).
+    // ranges, so it takes its place on a CU (two at dh up to 128, one above) as long as `worth` rows, of which as many run at a
+    // time as there are CUs; fewer tiles than places take no less time for that.  Over 2117 batches of 1 to 256 sequences and tokens, of
+    // like and unlike lengths up to 32768, 1 to 32 query heads to a kv head, 1 to 2 % from the faster one, the worst 1.17, 1.26, 1.49 times as
+    // long at dh 64, 128, 256.  Tiles against rows, dh 128: a step of 16 heads over 1 and 4096 keys 379 us, 109; 32 steps of 32
+    // over 8, 2000 to 4000 keys 455, 421; 16 tokens, 32 heads over 8, 32768 keys 3.42 ms, 1.76; 64 tokens 3.45, 5.88; 256
+    // tokens, 4096 keys 0.41, 2.59.
     const size_t cus = (size_t)op->dev->props.multiProcessorCount, rows = nt * (nh / nkvh), units = nkvh * ((rows + std::min(nseq, nt) * 63) / 64);
-    const size_t worth = dh <= 64 ? 2 : dh <= 128 ? 3 : 5;
-    const bool tiles = op->tile >= 0 ? op->tile > 0 : nt * nh >= worth * std::max(units, cus);
+    const double worth = dh <= 64 ? 2 : dh <= 128 ? 4.5 : 6;
+    const bool tiles = op->tile >= 0 ? op->tile > 0 : (double)(nt * nh) >= worth * (double)std::max(dh <= 128 ? units / 2 : units, cus);
     if (m.dt == OPHIP_DT_F32 && dh % 4 == 0 && dh <= 256 && p.b.cols && vec && units <= 0xffffffffu / 256 && tiles) {
         launch(op->f32[dh <= 64 ? 0 : dh <= 128 ? 1 : 2], Dim3{(unsigned)units}, Dim3{256}, 0, stream_of(qa), p);
         return;

@@ -1194,10 +1194,11 @@ def test_qk_norm_rope_refuses_results_over_what_it_reads(gpu, stream):
     (8, 1, 256, [(9, 100)], False),
     (4, 1, 64, [(16, 60)], False),              # 64 rows: one tile, or a workgroup for each
     (12, 4, 64, [(50, 50)], True),              # 600 rows in 12 tiles
-    (16, 2, 128, [(49, 50)], True),             # 784 rows
+    (16, 2, 128, [(49, 50)], False),            # 784 rows: at these sizes a row at a time is still faster
     (40, 1, 128, [(30, 40)], True),
-    (16, 2, 200, [(49, 50)], False),            # 784 rows: at this size a row at a time is still faster
-    (20, 1, 256, [(65, 65)], True),
+    (16, 2, 200, [(49, 50)], False),
+    (20, 1, 256, [(65, 65)], False),
+    (20, 1, 256, [(80, 80)], True),
 ], ids=str)
 def test_attention_paged_f32_tiles_only_where_they_fill_the_machine(gpu, stream, monkeypatch, nh, nkvh, dh, lens, tiles):
     """Tiles of 64 rows are never cut into ranges: few of them leave most CUs without work.  The chosen kernel shows in the
