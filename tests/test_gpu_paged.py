@@ -1327,3 +1327,75 @@ def test_attention_paged_few_and_many_key_ranges_of_256_rows(gpu, stream, monkey
     b = Batch(gpu, np.random.default_rng(74), "bf16", 4, 2, 128, 16, [(20, 2000), (1, 3000), (150, 900)])
     want, tol = b.expected(1)
     check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("dh,tile", [(64, "0"), (64, "1"), (128, "2"), (128, "3"), (96, "0"), (36, "0")])
+def test_attention_paged_subnormal_f16_values(gpu, stream, monkeypatch, dh, tile):
+    """Values and results below 2^-14, where f16 has steps of 2^-24: nothing is taken for zero."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(75), "f16", 4, 2, dh, 16, [(1, 1), (3, 40), (30, 64), (1, 300)])
+    small = decode(b.cache[1].host, "f16") * 2.0 ** -17
+    b.cache[1] = Buffer(gpu, encode(small, "f16"), "f16")
+    b.cache_views = [c.host for c in b.cache]
+    want, tol = b.expected(1)
+    assert np.abs(want).max() < 2.0 ** -14 and (np.abs(want) > tol).mean() > 0.9
+    check(attend(gpu, stream, b, 1), want, tol)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+def test_a_recorded_step_replayed_while_the_sequences_grow(gpu, kind):
+    """Norm and rotation, append and attention in one recorded graph, every replay bit for bit what the same calls give one by one on caches of
+    their own; inputs, positions, lengths and the table's entries are uploaded between replays."""
+    rng = np.random.default_rng(76)
+    nh, nkvh, dh, page, theta = 8, 2, 64, 16, 10000.0
+    cols, ns = 96, 3  # up to 1536 keys: wide enough for key ranges
+    pages = ns * cols
+    table = rng.permutation(pages).reshape(ns, cols).astype(np.uint32)
+    past = [encode(rng.standard_normal((pages, nkvh, page, dh)), kind) for _ in range(2)]
+    w = Buffer(gpu, encode(1 + 0.2 * rng.standard_normal(dh), "f32"), "f32")
+    ops = ophip.QkNormRope(gpu), ophip.KvAppendPaged(gpu), ophip.AttentionPaged(gpu)
+    sides = []
+    for _ in range(2):
+        s = {"qkv": Buffer(gpu, np.zeros((ns, (nh + 2 * nkvh) * dh), store(kind)), kind), "cache": [Buffer(gpu, c, kind) for c in past],
+             "o": Buffer(gpu, np.zeros((ns, nh, dh), store(kind)), kind), "table": Buffer(gpu, table), "start": Buffer(gpu, np.arange(ns + 1, dtype=np.uint32)),
+             "len": Buffer(gpu, np.zeros(ns, np.uint32)), "pos": Buffer(gpu, np.zeros(ns, np.uint32)), "stream": gpu.stream()}
+        heads = lambda a, h: np.lib.stride_tricks.as_strided(a, (ns, h, dh), (s["qkv"].host.strides[0], dh * SIZE[kind], SIZE[kind]))
+        q, k, v = heads(s["qkv"].host, nh), heads(s["qkv"].host[:, nh * dh:], nkvh), heads(s["qkv"].host[:, (nh + nkvh) * dh:], nkvh)
+        at = lambda x: s["qkv"].view(x)
+        batch, caches = s["table"].view() + s["start"].view() + s["len"].view(), s["cache"][0].view() + s["cache"][1].view()
+        s["args"] = (ophip.QkNormRopeArgs(*at(q), *at(q), *w.view(), *at(k), *at(k), *w.view(), *s["pos"].view(), 1e-6, theta),
+                     ophip.KvAppendPagedArgs(*at(k.transpose(1, 0, 2)), *at(v.transpose(1, 0, 2)), *s["pos"].view(), *caches, *batch, 0.0),
+                     ophip.AttentionPagedArgs(*at(q.transpose(1, 0, 2)), *caches, *s["o"].view(s["o"].host.transpose(1, 0, 2)), *batch, 1, dh ** -0.5))
+        s["ws"] = gpu.malloc(max(16, ops[2].scheme(s["args"][2], 1 << 40)))
+        sides.append(s)
+    recorded, eager = sides
+
+    def step(s):
+        for op, args, ws in zip(ops, s["args"], (None, None, s["ws"])):
+            op.launch(args, ws, s["stream"])
+
+    recorded["stream"].begin_capture()
+    step(recorded)
+    graph = recorded["stream"].end_capture()
+    lens = np.array([0, 700, 1500], np.uint32)
+    for turn in range(6):
+        lens = lens + 1
+        x = encode(rng.standard_normal((ns, (nh + 2 * nkvh) * dh)), kind)
+        if turn == 3:  # the sequences change places in the batch
+            lens, table = lens[::-1].copy(), table[::-1].copy()
+        for s in sides:
+            for name, value in (("qkv", x), ("len", lens), ("pos", lens - 1), ("table", table)):
+                gpu.upload(s[name].mem, np.ascontiguousarray(value))
+        graph.launch(recorded["stream"])
+        step(eager)
+        for s in sides:
+            s["stream"].synchronize()
+        for name in ("o", "qkv"):
+            a, b = (s[name].back(s["stream"]).view(np.uint8) for s in sides)
+            assert np.array_equal(a, b), "%s, replay %d" % (name, turn)
+        for a, b in zip(recorded["cache"], eager["cache"]):
+            assert np.array_equal(a.back(recorded["stream"]).view(np.uint8), b.back(eager["stream"]).view(np.uint8)), turn
+        assert np.isfinite(decode(eager["o"].back(eager["stream"]), kind)).all() and (decode(eager["o"].back(eager["stream"]), kind) != 0).any((1, 2)).all()
+    graph.destroy()
+    for s in sides:
+        s["stream"].destroy()
