@@ -507,19 +507,26 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
  *                    kv_len[s] - n + i.  Tokens in front of the first and behind the last sequence belong to none: their
  *                    rows are neither read nor written.
  * Table, starts and lengths are device data that may change between replays of a recorded launch.  The kernels bound
- * what they take from them: token numbers by nt, lengths by cols * page (attention) or keys (append); a page number that is none of the cache's
- * gets nothing written to, and reads as some page of the cache.  Wrong data gives wrong rows, not stray accesses.
+ * what they take from them: token numbers by nt; in attention lengths by cols * page, in append keys; a page number that
+ * is none of the cache's gets nothing written to, and reads as some page of the cache.  Wrong data gives wrong rows, not
+ * stray accesses.
  * Types: f16, bf16, f32, one for all tensors of a call.  dh up to 512. */
 
 /* attention of the new tokens over the cache: o = softmax(scale * q . k^T) . v, q and o [nh, nt, dh], nh a multiple of
  * nkvh (query head h reads kv head h / (nh / nkvh)).  With OPHIP_MASK_CAUSAL new token i of n sees the keys up to its
- * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero; one that sees keys, all of them with a score of
- * -inf, is NaN, as 0 / 0 is.  q is left alone; o may be q itself
- * (the same view), otherwise the address ranges of o and of q, the caches, the table, the starts or the lengths must not overlap (ArgsNotSupport).
- * What a row does not see does not touch it, infinite and NaN keys and values included.  Sums and softmax statistics are
- * f32; the result is rounded once, and in f16 and bf16 so are the probabilities of sequences with more than 16 rows
- * (new tokens times query heads per kv head).  Fast for f16 and bf16 with dh a multiple of 8 and f32
- * with dh a multiple of 4, up to 256, and rows that start on 16 bytes; other calls are right, but not fast. */
+ * own, kv_len - n + i; without, all kv_len.  A row that sees no key is zero; one that sees keys, all of them with a score
+ * of -inf, is NaN, as 0 / 0 is.  q is left alone; o may be q itself (the same view), otherwise the address ranges of o and
+ * of q, the caches, the table, the starts or the lengths must not overlap (ArgsNotSupport).
+ * What a row does not see does not touch it, infinite and NaN keys and values included.  (A value that is not finite costs
+ * time where some rows that are worked on together see it and others do not, and wherever a sequence of up to 16 rows sees it:
+ * those rows are worked through again key by key, up to some hundred times slower.)
+ * Sums and softmax statistics are f32; the result is rounded once, and in f16 and bf16 so are the probabilities of
+ * sequences with more than 16 rows (new tokens times query heads per kv head), in f16 those below 2^-32 of the largest to zero.
+ * Which kernel a sequence runs on depends on the sizes of the whole call: so do the order of its sums and, with more than 16
+ * rows, whether its probabilities are rounded.  Kernels and key ranges are chosen by cols * page, not by the lengths, which
+ * the host does not know.
+ * Fast for f16 and bf16 with dh a multiple of 8 and f32 with dh a multiple of 4, up to 256, and rows that start on 16
+ * bytes; other calls are right, but not fast. */
 typedef struct ophip_attention_paged_args {
     ophip_tensor_layout q_layout;
     const void *q_base;

@@ -112,7 +112,7 @@ __device__ __forceinline__ void paged_exactly(const AttnPagedParams &p, const Pa
 //   which the lane reads DH / 16 adjacent columns each and transposes them in registers.
 // The matrix cores are idle most of the time: 16 KB of keys and values take about 500 cycles of one wave, a CU's share of
 // the memory's rate delivers them in 1300.  Memory bounds it: 50 decode steps over 165008 keys, 8 kv heads of 128, 676 MB,
-// 118 us, 5.75 TB/s (a pure read of that size with the non-temporal hint 6.46, a copy 4.89); below some 50 MB the latencies of the
+// 116 us, 5.8 TB/s (a pure read of that size with the non-temporal hint 6.46, a copy 4.89); below some 50 MB the latencies of the
 // launches, the plan and a range's first loads do (one step over 2047 keys, 8 MB: 11 us, of which 9 are the two launches).
 template <int CW>
 struct FewTile {  // 32 keys
@@ -338,11 +338,11 @@ __device__ __forceinline__ void paged_few(const AttnPagedParams &p, const PagedI
 // registers into B operands of O^T = V^T . P^T, whose A operands come from the row-major tile through the transposing
 // LDS read.  A wave without rows, or whose rows all end before a tile, only helps to load.
 // What bounds it is the matrix cores' rate together with the exponentials that their order leaves between the products: 8192
-// tokens, 32 heads over 8 of 128, causal, 0.55 Tflop kept: 565 us, 0.97 PF (a plain product of 8192^3 reaches 1.24) with eight
-// waves that share a tile's loads, 602 with four; 511 tokens over 32511 keys 290 us, 0.93 PF (machines differ by a tenth).  In
-// the order that the compiler gives them, products, LDS reads and the second half's exponentials took 633 us where the one
+// tokens, 32 heads over 8 of 128, causal, 0.55 Tflop kept: 552 us, 1.0 PF (a plain product of 8192^3 reaches 1.26) with eight
+// waves that share a tile's loads (565 against 602 with four on one machine); 511 tokens over 32511 keys 275 us, 0.98 PF (machines
+// differ by a tenth).  In the order that the compiler gives them, products, LDS reads and the second half's exponentials took 633 us where the one
 // below took 593; a raised priority of the wave around its products changed nothing.  Short prompts are bound by a unit's
-// fixed time, some 6 us: 7 prompts of 104 to 546 tokens, 32 heads of 128: 30 us.
+// fixed time, some 6 us, and by the longest tiles, two of which share a CU: 7 prompts of 104 to 546 tokens, 32 heads of 128: 26 us.
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int DH>

@@ -1,4 +1,4 @@
-// attention over a paged cache for what the matrix kernels (attention_paged.hip, attention_paged_f32.hip) do not take: decode steps in
+// attention over a paged cache for what the matrix kernels (attention_paged.hip, attention_paged_f32.hip) do not take: few rows in
 // f32, head dimensions other than theirs, elements that are not adjacent, addresses that are not 16-byte aligned.
 //
 // One workgroup per token and query head.  A wave takes U keys at a time, every WAVES-th such group, and requests all their
@@ -7,7 +7,7 @@
 // softmax's maximum is then taken, and its powers, once for every key and not in every lane.  The waves' maxima, sums
 // and outputs are joined in LDS.  Every key is read once per query head and token, from the caches where it
 // was read before; what bounds the kernel is instructions for many tokens and latency for few, which then get sixteen waves.
-// f32, 32 heads over 8 of 128 columns: a decode step over 2048 keys 60 us, 32 of them over 2000 to 4000 keys 414 us (790 MB,
+// f32, 32 heads over 8 of 128 columns: a decode step over 2048 keys 61 us, 32 of them over 2000 to 4000 keys 422 us (790 MB,
 // 1.9 TB/s), 2048 tokens with rows off 16 bytes 5.3 ms (with one key at a time 839 us, 2.3 ms, 11.6 ms).
 #include "paged.h"
 

@@ -1,4 +1,4 @@
-// attention over a paged cache in f32 on the matrix cores, for sequences with more than a few rows: o = softmax(scale q . k^T) . v,
+// attention over a paged cache in f32 on the matrix cores, for enough rows to fill the machine with tiles (the host chooses): o = softmax(scale q . k^T) . v,
 // head dimensions of a multiple of 4 up to 256 (kernels for 64, 128 and 256 columns, the missing ones zero).
 //
 // A workgroup takes 64 rows of a sequence and kv head (row = token * group + head-in-group), 16 to each of its four waves, and
@@ -9,7 +9,8 @@
 //   O^T = V^T . P^T.  Its rows are free as well: row r of block d is column 64 (d / 4) + 4 r + d % 4, so that a lane reads 16 bytes of
 //   a value for four blocks, and stores 16 bytes of the result.
 // The matrix cores bound it: 157 Tflop/s in f32, a sixteenth of what they do in f16.  2048 tokens, 32 heads over 8 of 128, causal,
-// 34 Gflop kept: 393 us, 0.09 Pflop/s (a row at a time, attention_paged_any.hip, 5.3 ms); 512 tokens 59 us.
+// 34 Gflop kept: 396 us, 0.09 Pflop/s (a row at a time, attention_paged_any.hip, 5.3 ms); 512 tokens 59 us.  A tile's keys are
+// not cut into ranges: 256 tokens over 8256 keys are 128 workgroups on 256 CUs, 839 us.
 #include "paged_plan.h"
 
 template <int DH>
