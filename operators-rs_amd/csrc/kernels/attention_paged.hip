@@ -520,6 +520,8 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             }
             const float shift = PA_BIAS - (m == -INFINITY ? 0.f : m);  // (a row that has kept nothing so far: every term is 0)
             PackE pb[4];  // MFMA n: the tile's keys 16 n .. + 15, slots 8 h .. 8 h + 7 keys 16 n + 4 h + {0..3}, 16 n + 8 + 4 h + {0..3}
+            // Rounded to the type for the product, added up as they are: a second product for the rest, as in paged_few, would be half as
+            // much again of the matrix cores' work, which bounds the kernel.  Errors against 64 bits are 1.2 to 1.4 times those of f32 ones.
             auto power = [&](int b, int e) {
                 const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift));
                 l += x;
