@@ -521,7 +521,8 @@ OPHIP_API void ophip_attention_kv_cached_destroy(ophip_attention_kv_cached *op);
  * time where some rows that are worked on together see it and others do not, and wherever a sequence of up to 16 rows sees it:
  * those rows are worked through again key by key, up to some hundred times slower.)
  * Sums and softmax statistics are f32; the result is rounded once, and in f16 and bf16 so are the probabilities of
- * sequences with more than 16 rows (new tokens times query heads per kv head), in f16 those below 2^-32 of the largest to zero.
+ * sequences with more than 16 rows (new tokens times query heads per kv head), in f16 those below 2^-32 of the largest to zero; they are
+ * divided by the sum of the rounded ones.
  * Which kernel a sequence runs on depends on the sizes of the whole call: so do the order of its sums and, with more than 16
  * rows, whether its probabilities are rounded.  Kernels and key ranges are chosen by cols * page, not by the lengths, which
  * the host does not know.

@@ -51,6 +51,17 @@ __device__ __forceinline__ bool not_finite(uint32_t most) {
     return (most & 0xffffu) >= ONES || (most >> 16) >= ONES;
 }
 
+// sum + the pair's two elements (v_dot2c: subnormal ones count, f32 rounding)
+__device__ __forceinline__ float add_pair(float sum, uint32_t pair) {
+    typedef elem elem2 __attribute__((ext_vector_type(2)));
+    const elem2 x = __builtin_bit_cast(elem2, pair), one = {(elem)1.f, (elem)1.f};
+#ifdef GEMM_ELEM_BF16
+    return __builtin_amdgcn_fdot2_f32_bf16(x, one, sum, false);
+#else
+    return __builtin_amdgcn_fdot2(x, one, sum, false);
+#endif
+}
+
 // The matrix kernels multiply the values of a tile's keys with a probability of zero where a row does not keep them, and
 // zero times infinity or NaN is NaN.  Where paged_many has met values that are not finite in a tile that some row keeps in part
 // (the last ones under a causal mask), and where paged_few's sums are not finite, they come here for the whole range instead
@@ -520,12 +531,14 @@ __device__ __forceinline__ void paged_many(const AttnPagedParams &p, const Paged
             }
             const float shift = PA_BIAS - (m == -INFINITY ? 0.f : m);  // (a row that has kept nothing so far: every term is 0)
             PackE pb[4];  // MFMA n: the tile's keys 16 n .. + 15, slots 8 h .. 8 h + 7 keys 16 n + 4 h + {0..3}, 16 n + 8 + 4 h + {0..3}
-            // Rounded to the type for the product, added up as they are: a second product for the rest, as in paged_few, would be half as
-            // much again of the matrix cores' work, which bounds the kernel.  Errors against 64 bits are 1.2 to 1.4 times those of f32 ones.
+            // Rounded to the type for the product: a second product for the rest, as in paged_few, would be half as much again of the matrix
+            // cores' work, which bounds the kernel; errors against 64 bits are 1.2 to 1.4 times those of f32 probabilities.  The sum is of the
+            // rounded ones, so that a row stays a mean of its values (with the sum of the others rows of f16's largest value came out
+            // infinite); the pair's sum is one instruction (8192 tokens 556 us; a conversion and an addition for each 595).
             auto power = [&](int b, int e) {
-                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift));
-                l += x;
-                pb[2 * b + e / 8].e[e % 8] = f2e(x);
+                PackE &eight = pb[2 * b + e / 8];
+                eight.e[e % 8] = f2e(__builtin_amdgcn_exp2f(__builtin_fmaf(sacc[b][e], scale2, shift)));
+                if (e % 2) l = add_pair(l, eight.u[e % 8 / 2]);
             };
             typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
             {

@@ -78,6 +78,9 @@ inline double rsqrt(double x) { return 1.0 / sqrt(x); }
 #define __builtin_amdgcn_sched_group_barrier(a, b, c) ((void)0)
 #define __builtin_amdgcn_fence(order, scope) std::atomic_thread_fence(std::memory_order_seq_cst)
 #define __builtin_amdgcn_exp2f(x) exp2f(x)
+// v_dot2_f32_{f16,bf16}: c + a . b over two elements
+#define __builtin_amdgcn_fdot2(a, b, c, clamp) ((float)(a)[1] * (float)(b)[1] + ((float)(a)[0] * (float)(b)[0] + (c)))
+#define __builtin_amdgcn_fdot2_f32_bf16(a, b, c, clamp) __builtin_amdgcn_fdot2(a, b, c, clamp)
 #define __builtin_amdgcn_rcpf(x) (1.0f / (x))
 #define __builtin_amdgcn_s_setprio(x) ((void)0)
 

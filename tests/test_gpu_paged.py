@@ -1399,3 +1399,24 @@ def test_a_recorded_step_replayed_while_the_sequences_grow(gpu, kind):
     graph.destroy()
     for s in sides:
         s["stream"].destroy()
+
+
+# ---- a row is a mean of values: it does not leave their range
+
+@pytest.mark.parametrize("kind,dh,tile", EVERY_KERNEL)
+@pytest.mark.parametrize("value", [1.0, 65504.0, -65504.0])
+@pytest.mark.parametrize("spread", [1.0, 4.0])
+def test_attention_paged_values_that_are_all_the_same(gpu, stream, monkeypatch, kind, dh, tile, value, spread):
+    """Whatever the probabilities, rounded or not: their sum is what they are divided by.  One rounding of the result, the second order of the
+    rests (u^2), and the additions of K like-signed terms in f32, each off by e of a sum that is no larger than the last, in the numerator
+    and in the sum of probabilities: (u + u^2 + 2 K e) |c|; at the largest value of f16 as well, next to which infinity lies."""
+    monkeypatch.setenv("OPHIP_ATTN_PAGED_TILE", tile)
+    b = Batch(gpu, np.random.default_rng(77), kind, 4, 2, dh, 16, [(30, 64), (90, 90), (1, 50), (20, 1200), (5, 3), (40, 41)], junk=0.0)
+    b.q = Buffer(gpu, encode(decode(b.q.host, kind) * spread, kind), kind)
+    c = float(decode(encode(np.array([value]), kind), kind)[0])
+    b.cache[1] = Buffer(gpu, encode(np.full(b.cache[1].host.shape, c), kind), kind)
+    b.cache_views = [x.host for x in b.cache]
+    want = np.full((b.nt, b.nh, dh), c)
+    want[b.start[4]:b.start[4] + 2] = 0  # no key
+    u = HALF[kind]
+    check(attend(gpu, stream, b, 1), want, (u + u * u + 2 * 1200 * E) * np.abs(want))
